@@ -718,6 +718,312 @@ at::Tensor indice_maxpool_backward(const at::Tensor& features_in, const at::Tens
   return gx;
 }
 
+// ------------------------------------------------ attention-block operators
+namespace {
+
+// [T, H, D] with its rows where the kernels can read them in 16-byte steps:
+// innermost stride 1, row and head strides and the base on 16 bytes, no
+// broadcast (zero) stride.  Anything else is copied.
+struct Heads {
+  at::Tensor t;
+  int64_t row, head;
+};
+
+Heads heads_of(const at::Tensor& in, const char* name, bool contiguous = false) {
+  TORCH_CHECK_VALUE(in.dim() == 3, name, " must be [tokens, heads, dim]");
+  const int64_t per16 = std::max<int64_t>(1, 16 / (int64_t)in.element_size());
+  const int64_t d = in.size(2), dense = in.size(1) * d;
+  auto strides = [&](const at::Tensor& t, int64_t* row, int64_t* head) {
+    *head = t.size(1) == 1 ? d : t.stride(1);  // the stride of a single head or row says nothing
+    *row = t.size(0) <= 1 ? dense : t.stride(0);
+  };
+  Heads h{in, 0, 0};
+  strides(in, &h.row, &h.head);
+  const bool ok = (d <= 1 || in.stride(2) == 1) && h.row > 0 && h.head > 0 && h.row % per16 == 0 &&
+                  h.head % per16 == 0 && reinterpret_cast<uintptr_t>(in.data_ptr()) % 16 == 0 &&
+                  (!contiguous || (h.head == d && h.row == dense));
+  if (!ok) {
+    h.t = at::empty(in.sizes(), in.options().memory_format(at::MemoryFormat::Contiguous)).copy_(in);
+    h.row = dense;
+    h.head = d;
+  }
+  return h;
+}
+
+at::Tensor offsets_of(const at::Tensor& in, const char* name, const at::Tensor& like) {
+  require_cuda(in, name);
+  TORCH_CHECK(in.device() == like.device(), name, " must be on the device of q");
+  TORCH_CHECK_VALUE(in.dim() == 1, name, " must be one-dimensional");
+  TORCH_CHECK_TYPE(in.scalar_type() == at::kInt || in.scalar_type() == at::kLong, name, " must be int32 or int64");
+  return in.to(at::kInt).contiguous();
+}
+
+struct Packed {
+  Heads q, k, v;
+  at::Tensor cu_q, cu_k, lengths;
+  int64_t strides[6];
+  int64_t total_q, total_k, heads, kv_heads, dim, seqs;
+  int dtype;
+  const int32_t* lengths_ptr() const { return lengths.defined() ? lengths.data_ptr<int32_t>() : nullptr; }
+};
+
+Packed packed_of(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& cu_q,
+                 const at::Tensor& cu_k, const c10::optional<at::Tensor>& kv_lengths) {
+  require_cuda(k, "k");
+  require_cuda(v, "v");
+  TORCH_CHECK(k.device() == q.device() && v.device() == q.device(), "q, k and v must be on one device");
+  TORCH_CHECK_TYPE(q.scalar_type() == at::kHalf || q.scalar_type() == at::kBFloat16,
+                   "q must be float16 or bfloat16, got ", q.scalar_type());
+  TORCH_CHECK_TYPE(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(),
+                   "k and v must have the dtype of q");
+  Packed p;
+  p.q = heads_of(q, "q");
+  p.k = heads_of(k, "k");
+  p.v = heads_of(v, "v");
+  p.total_q = q.size(0), p.total_k = k.size(0), p.heads = q.size(1), p.kv_heads = k.size(1), p.dim = q.size(2);
+  TORCH_CHECK_VALUE(k.size(2) == p.dim && v.sizes() == k.sizes(), "k and v must be [keys, kv_heads, dim of q]");
+  TORCH_CHECK_VALUE(p.dim >= 8 && p.dim <= 128 && p.dim % 8 == 0, "dim must be a multiple of 8 up to 128, got ",
+                    p.dim);
+  TORCH_CHECK_VALUE(p.kv_heads >= 1 && p.heads >= 1 && p.heads % p.kv_heads == 0,
+                    "the query heads (", p.heads, ") must be a multiple of the key heads (", p.kv_heads, ")");
+  p.cu_q = offsets_of(cu_q, "cu_seqlens_q", q);
+  p.cu_k = offsets_of(cu_k, "cu_seqlens_k", q);
+  TORCH_CHECK_VALUE(p.cu_q.numel() >= 1 && p.cu_q.numel() == p.cu_k.numel(),
+                    "cu_seqlens_q and cu_seqlens_k must hold one offset more than there are sequences, got ",
+                    p.cu_q.numel(), " and ", p.cu_k.numel());
+  p.seqs = p.cu_q.numel() - 1;
+  if (kv_lengths.has_value() && kv_lengths->defined()) {
+    p.lengths = offsets_of(*kv_lengths, "kv_lengths", q);
+    TORCH_CHECK_VALUE(p.lengths.numel() == p.seqs, "kv_lengths must hold one length for each of the ", p.seqs,
+                      " sequences, got ", p.lengths.numel());
+  }
+  const int64_t s[6] = {p.q.row, p.q.head, p.k.row, p.k.head, p.v.row, p.v.head};
+  std::copy(s, s + 6, p.strides);
+  p.dtype = dtype_code(q);
+  return p;
+}
+
+at::Tensor attention_workspace(const Packed& p, int backward) {
+  size_t bytes = 0;
+  check(bfb_packed_attention_workspace_size(p.total_q, p.total_k, p.heads, p.kv_heads, p.dim, p.seqs, backward, &bytes),
+        "packed_attention workspace query");
+  return at::empty({(int64_t)bytes}, p.q.t.options().dtype(at::kByte));
+}
+
+}  // namespace
+
+std::tuple<at::Tensor, at::Tensor> packed_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                                    const at::Tensor& cu_q, const at::Tensor& cu_k,
+                                                    const c10::optional<at::Tensor>& kv_lengths, bool causal,
+                                                    double scale) {
+  NvtxRange nvtx_("bfb_b200::packed_attention");
+  require_cuda(q, "q");
+  c10::cuda::CUDAGuard guard(q.device());
+  const Packed p = packed_of(q, k, v, cu_q, cu_k, kv_lengths);
+  auto out = at::empty({p.total_q, p.heads, p.dim}, q.options().memory_format(at::MemoryFormat::Contiguous));
+  auto lse = at::empty({p.heads, p.total_q}, out.options().dtype(at::kFloat));
+  auto ws = attention_workspace(p, 0);
+  check(bfb_packed_attention(p.q.t.data_ptr(), p.k.t.data_ptr(), p.v.t.data_ptr(), p.strides, p.dtype, p.total_q,
+                             p.total_k, p.heads, p.kv_heads, p.dim, p.seqs, p.cu_q.data_ptr<int32_t>(),
+                             p.cu_k.data_ptr<int32_t>(), p.lengths_ptr(), causal ? 1 : 0, scale, out.data_ptr(),
+                             lse.data_ptr<float>(), ws.data_ptr(), (size_t)ws.numel(), stream_of(q)),
+        "packed_attention");
+  return {out, lse};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> packed_attention_backward(
+    const at::Tensor& out_grad, const c10::optional<at::Tensor>& lse_grad, const at::Tensor& q, const at::Tensor& k,
+    const at::Tensor& v, const at::Tensor& out, const at::Tensor& lse, const at::Tensor& cu_q, const at::Tensor& cu_k,
+    const c10::optional<at::Tensor>& kv_lengths, bool causal, double scale) {
+  NvtxRange nvtx_("bfb_b200::packed_attention_backward");
+  require_cuda(q, "q");
+  c10::cuda::CUDAGuard guard(q.device());
+  const Packed p = packed_of(q, k, v, cu_q, cu_k, kv_lengths);
+  require_cuda(out_grad, "out_grad");
+  TORCH_CHECK_VALUE(out_grad.sizes() == q.sizes() && out.sizes() == q.sizes(), "out and its gradient must match q");
+  TORCH_CHECK_VALUE(lse.dim() == 2 && lse.size(0) == p.heads && lse.size(1) == p.total_q &&
+                        lse.scalar_type() == at::kFloat,
+                    "lse must be float32 [heads, queries]");
+  const auto dout = heads_of(out_grad.to(q.scalar_type()), "out_grad", true).t;
+  const auto o = heads_of(out, "out", true).t;
+  const auto l = lse.contiguous();
+  at::Tensor dlse;
+  if (lse_grad.has_value() && lse_grad->defined()) {
+    TORCH_CHECK_VALUE(lse_grad->sizes() == lse.sizes(), "the gradient of lse must match it");
+    dlse = lse_grad->to(at::kFloat).contiguous();
+  }
+  auto dq = at::empty(q.sizes(), out.options().memory_format(at::MemoryFormat::Contiguous));
+  auto dk = at::empty(k.sizes(), dq.options()), dv = at::empty(v.sizes(), dq.options());
+  auto ws = attention_workspace(p, 1);
+  check(bfb_packed_attention_backward(
+            dout.data_ptr(), dlse.defined() ? dlse.data_ptr<float>() : nullptr, p.q.t.data_ptr(), p.k.t.data_ptr(),
+            p.v.t.data_ptr(), p.strides, o.data_ptr(), l.data_ptr<float>(), p.dtype, p.total_q, p.total_k, p.heads,
+            p.kv_heads, p.dim, p.seqs, p.cu_q.data_ptr<int32_t>(), p.cu_k.data_ptr<int32_t>(), p.lengths_ptr(),
+            causal ? 1 : 0, scale, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), ws.data_ptr(), (size_t)ws.numel(),
+            stream_of(q)),
+        "packed_attention_backward");
+  return {dq, dk, dv};
+}
+
+namespace {
+
+struct Rotary {
+  Heads q, k;
+  at::Tensor positions, freq, qw, kw;
+  std::vector<int64_t> sections;
+  int position_type;
+  int64_t rotated;
+};
+
+Rotary rotary_of(const at::Tensor& q, const at::Tensor& k, const at::Tensor& positions, const at::Tensor& inv_freq,
+                 at::IntArrayRef sections, const c10::optional<at::Tensor>& q_weight,
+                 const c10::optional<at::Tensor>& k_weight, bool interleaved) {
+  require_cuda(k, "k");
+  require_cuda(positions, "positions");
+  require_cuda(inv_freq, "inv_freq");
+  TORCH_CHECK(k.device() == q.device() && positions.device() == q.device() && inv_freq.device() == q.device(),
+              "q, k, positions and inv_freq must be on one device");
+  Rotary r;
+  (void)dtype_code(q);
+  TORCH_CHECK_TYPE(k.scalar_type() == q.scalar_type(), "k must have the dtype of q");
+  r.q = heads_of(q, "q");
+  r.k = heads_of(k, "k");
+  const int64_t dim = q.size(2);
+  TORCH_CHECK_VALUE(k.size(0) == q.size(0) && k.size(2) == dim, "k must have the tokens and the dim of q");
+  TORCH_CHECK_VALUE(q.size(1) >= 1 && k.size(1) >= 1, "q and k need at least one head");
+  TORCH_CHECK_VALUE(dim >= 8 && dim <= 256 && dim % 8 == 0, "dim must be a multiple of 8 up to 256, got ", dim);
+  TORCH_CHECK_VALUE(!sections.empty() && sections.size() <= 8, "sections must name 1 to 8 axes");
+  r.sections = sections.vec();
+  int64_t pairs = 0;
+  for (const int64_t s : r.sections) {
+    TORCH_CHECK_VALUE(s >= 0 && s <= dim, "sections must not be negative");
+    pairs += s;
+  }
+  r.rotated = 2 * pairs;
+  TORCH_CHECK_VALUE(pairs >= 1 && r.rotated <= dim && r.rotated % (interleaved ? 2 : 16) == 0,
+                    "the sections' sum must be at least 1, at most dim / 2",
+                    interleaved ? "" : " and (pairs half the rotated width apart) a multiple of 8", ", got ", pairs);
+  TORCH_CHECK_VALUE(inv_freq.dim() == 1 && inv_freq.size(0) == pairs, "inv_freq must hold the sections' sum of ",
+                    pairs, " values");
+  TORCH_CHECK_TYPE(inv_freq.scalar_type() == at::kFloat || inv_freq.scalar_type() == at::kDouble,
+                   "inv_freq must be float32 or float64");
+  TORCH_CHECK_VALUE(positions.dim() == 2 && positions.size(0) == q.size(0) &&
+                        positions.size(1) == (int64_t)r.sections.size(),
+                    "positions must be [tokens, axes]");
+  switch (positions.scalar_type()) {
+    case at::kInt: r.position_type = 0; break;
+    case at::kLong: r.position_type = 1; break;
+    case at::kFloat: r.position_type = 2; break;
+    default: TORCH_CHECK_TYPE(false, "positions must be int32, int64 or float32, got ", positions.scalar_type());
+  }
+  r.positions = positions;
+  r.freq = inv_freq.contiguous();
+  auto weight = [&](const c10::optional<at::Tensor>& w, const char* name) -> at::Tensor {
+    if (!w.has_value() || !w->defined()) return {};
+    require_cuda(*w, name);
+    TORCH_CHECK(w->device() == q.device(), name, " must be on the device of q");
+    TORCH_CHECK_TYPE(w->scalar_type() == at::kFloat, name, " must be float32");
+    TORCH_CHECK_VALUE(w->dim() == 1 && w->size(0) == dim, name, " must be [dim]");
+    auto c = w->contiguous();
+    return reinterpret_cast<uintptr_t>(c.data_ptr()) % 16 ? c.clone() : c;
+  };
+  r.qw = weight(q_weight, "q_weight");
+  r.kw = weight(k_weight, "k_weight");
+  return r;
+}
+
+const float* floats_or_null(const at::Tensor& t) { return t.defined() ? t.data_ptr<float>() : nullptr; }
+
+}  // namespace
+
+std::tuple<at::Tensor, at::Tensor> qk_norm_rotary(const at::Tensor& q, const at::Tensor& k,
+                                                  const at::Tensor& positions, const at::Tensor& inv_freq,
+                                                  at::IntArrayRef sections, const c10::optional<at::Tensor>& q_weight,
+                                                  const c10::optional<at::Tensor>& k_weight, double eps,
+                                                  bool interleaved) {
+  NvtxRange nvtx_("bfb_b200::qk_norm_rotary");
+  require_cuda(q, "q");
+  c10::cuda::CUDAGuard guard(q.device());
+  const Rotary r = rotary_of(q, k, positions, inv_freq, sections, q_weight, k_weight, interleaved);
+  auto qo = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
+  auto ko = at::empty(k.sizes(), qo.options());
+  check(bfb_qk_norm_rotary(r.q.t.data_ptr(), r.k.t.data_ptr(), r.q.row, r.q.head, r.k.row, r.k.head, dtype_code(q),
+                           q.size(0), q.size(1), k.size(1), q.size(2), r.rotated, r.positions.data_ptr(),
+                           r.position_type, r.positions.stride(0), r.positions.stride(1), r.freq.data_ptr(),
+                           r.freq.scalar_type() == at::kDouble, (int64_t)r.sections.size(), r.sections.data(),
+                           floats_or_null(r.qw), floats_or_null(r.kw), eps, interleaved ? 1 : 0, qo.data_ptr(),
+                           ko.data_ptr(), stream_of(q)),
+        "qk_norm_rotary");
+  return {qo, ko};
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> qk_norm_rotary_backward(
+    const at::Tensor& q_grad, const at::Tensor& k_grad, const at::Tensor& q, const at::Tensor& k,
+    const at::Tensor& positions, const at::Tensor& inv_freq, at::IntArrayRef sections,
+    const c10::optional<at::Tensor>& q_weight, const c10::optional<at::Tensor>& k_weight, double eps,
+    bool interleaved) {
+  NvtxRange nvtx_("bfb_b200::qk_norm_rotary_backward");
+  require_cuda(q, "q");
+  c10::cuda::CUDAGuard guard(q.device());
+  const Rotary r = rotary_of(q, k, positions, inv_freq, sections, q_weight, k_weight, interleaved);
+  require_cuda(q_grad, "q_grad");
+  require_cuda(k_grad, "k_grad");
+  TORCH_CHECK_VALUE(q_grad.sizes() == q.sizes() && k_grad.sizes() == k.sizes(),
+                    "the outputs' gradients must match q and k");
+  const auto gq = heads_of(q_grad.to(q.scalar_type()), "q_grad", true).t;
+  const auto gk = heads_of(k_grad.to(q.scalar_type()), "k_grad", true).t;
+  auto dq = at::empty(q.sizes(), q.options().memory_format(at::MemoryFormat::Contiguous));
+  auto dk = at::empty(k.sizes(), dq.options());
+  auto weight_grad = [&](const at::Tensor& w) {
+    return at::empty({w.defined() ? q.size(2) : 0}, dq.options().dtype(at::kFloat));
+  };
+  auto dqw = weight_grad(r.qw), dkw = weight_grad(r.kw);
+  at::Tensor ws;
+  size_t bytes = 0;
+  if (r.qw.defined() || r.kw.defined()) {
+    check(bfb_qk_norm_rotary_backward_workspace_size(q.size(2), &bytes), "qk_norm_rotary workspace query");
+    ws = at::empty({(int64_t)bytes}, dq.options().dtype(at::kByte));
+  }
+  check(bfb_qk_norm_rotary_backward(
+            gq.data_ptr(), gk.data_ptr(), r.q.t.data_ptr(), r.k.t.data_ptr(), r.q.row, r.q.head, r.k.row, r.k.head,
+            dtype_code(q), q.size(0), q.size(1), k.size(1), q.size(2), r.rotated, r.positions.data_ptr(),
+            r.position_type, r.positions.stride(0), r.positions.stride(1), r.freq.data_ptr(),
+            r.freq.scalar_type() == at::kDouble, (int64_t)r.sections.size(), r.sections.data(), floats_or_null(r.qw),
+            floats_or_null(r.kw), eps, interleaved ? 1 : 0, dq.data_ptr(), dk.data_ptr(),
+            r.qw.defined() ? dqw.data_ptr<float>() : nullptr, r.kw.defined() ? dkw.data_ptr<float>() : nullptr,
+            ws.defined() ? ws.data_ptr() : nullptr, bytes, stream_of(q)),
+        "qk_norm_rotary_backward");
+  return {dq, dk, dqw, dkw};
+}
+
+at::Tensor residual_dropout(const at::Tensor& x_in, const c10::optional<at::Tensor>& residual_in, double p,
+                            const at::Tensor& seed) {
+  NvtxRange nvtx_("bfb_b200::residual_dropout");
+  require_cuda(x_in, "x");
+  c10::cuda::CUDAGuard guard(x_in.device());
+  const int dt = dtype_code(x_in);
+  TORCH_CHECK_VALUE(p >= 0.0 && p <= 1.0, "p must be a probability, got ", p);
+  require_cuda(seed, "seed");
+  TORCH_CHECK(seed.device() == x_in.device(), "seed must be on the device of x");
+  TORCH_CHECK_TYPE(seed.scalar_type() == at::kLong, "seed must be int64");
+  TORCH_CHECK_VALUE(seed.numel() == 2, "seed must hold two values");
+  auto x = x_in.contiguous();
+  auto s = seed.contiguous();
+  at::Tensor residual;
+  if (residual_in.has_value() && residual_in->defined()) {
+    require_cuda(*residual_in, "residual");
+    TORCH_CHECK(residual_in->device() == x.device(), "residual must be on the device of x");
+    TORCH_CHECK_TYPE(residual_in->scalar_type() == x.scalar_type(), "residual must have the dtype of x");
+    TORCH_CHECK_VALUE(residual_in->sizes() == x.sizes(), "residual must have the shape of x");
+    residual = residual_in->contiguous();
+  }
+  auto out = at::empty(x.sizes(), x.options().memory_format(at::MemoryFormat::Contiguous));
+  check(bfb_residual_dropout(x.data_ptr(), residual.defined() ? residual.data_ptr() : nullptr, dt, x.numel(),
+                             s.data_ptr<int64_t>(), p, out.data_ptr(), stream_of(x)),
+        "residual_dropout");
+  return out;
+}
+
 TORCH_LIBRARY(bfb_b200, m) {
   m.def("bev_pool_forward(Tensor feats, Tensor coords, int B, int D, int H, int W) -> (Tensor, Tensor)");
   m.def("bev_pool_plan(Tensor coords, int B, int D, int H, int W) -> Tensor");
@@ -764,6 +1070,21 @@ TORCH_LIBRARY(bfb_b200, m) {
   m.def(
       "indice_maxpool_backward(Tensor features, Tensor out_features, Tensor out_bp, Tensor indice_pairs, "
       "Tensor indice_pair_num) -> Tensor");
+  m.def(
+      "packed_attention(Tensor q, Tensor k, Tensor v, Tensor cu_seqlens_q, Tensor cu_seqlens_k, Tensor? kv_lengths, "
+      "bool causal, float scale) -> (Tensor, Tensor)");
+  m.def(
+      "packed_attention_backward(Tensor out_grad, Tensor? lse_grad, Tensor q, Tensor k, Tensor v, Tensor out, "
+      "Tensor lse, Tensor cu_seqlens_q, Tensor cu_seqlens_k, Tensor? kv_lengths, bool causal, float scale) -> "
+      "(Tensor, Tensor, Tensor)");
+  m.def(
+      "qk_norm_rotary(Tensor q, Tensor k, Tensor positions, Tensor inv_freq, int[] sections, Tensor? q_weight, "
+      "Tensor? k_weight, float eps, bool interleaved) -> (Tensor, Tensor)");
+  m.def(
+      "qk_norm_rotary_backward(Tensor q_grad, Tensor k_grad, Tensor q, Tensor k, Tensor positions, Tensor inv_freq, "
+      "int[] sections, Tensor? q_weight, Tensor? k_weight, float eps, bool interleaved) -> (Tensor, Tensor, Tensor, "
+      "Tensor)");
+  m.def("residual_dropout(Tensor x, Tensor? residual, float p, Tensor seed) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(bfb_b200, CUDA, m) {
@@ -789,4 +1110,9 @@ TORCH_LIBRARY_IMPL(bfb_b200, CUDA, m) {
   m.impl("indice_conv_backward", &indice_conv_backward);
   m.impl("indice_maxpool", &indice_maxpool);
   m.impl("indice_maxpool_backward", &indice_maxpool_backward);
+  m.impl("packed_attention", &packed_attention);
+  m.impl("packed_attention_backward", &packed_attention_backward);
+  m.impl("qk_norm_rotary", &qk_norm_rotary);
+  m.impl("qk_norm_rotary_backward", &qk_norm_rotary_backward);
+  m.impl("residual_dropout", &residual_dropout);
 }

@@ -474,6 +474,92 @@ int bfb_indice_maxpool_backward(const void* features_dev, const void* out_featur
  * a correct run); reset = 1 clears it.  No reference counterpart. */
 int bfb_spconv_timeouts(uint64_t* count, int reset);
 
+/* ------------------------------------------------------------------------
+ * Attention-block operators over active sites (no reference counterpart):
+ * packed attention, the norm of query and key heads with their rotary
+ * positions, and dropout onto the residual stream.
+ *
+ * Packed attention.  q [total_q, heads, dim], k and v [total_k, kv_heads,
+ * dim], f16 or bf16, dim a multiple of 8 up to 128, heads a multiple of
+ * kv_heads (query head h reads key head h / (heads / kv_heads)).  `strides`
+ * (HOST, 6 values, elements): row and head strides of q, k and v; they and
+ * the base addresses are multiples of 16 bytes, the innermost stride is 1.
+ * cu_q, cu_k [seqs + 1] int32: sequence s holds the query rows cu_q[s] ..
+ * cu_q[s + 1] - 1 and the key rows cu_k[s] .. cu_k[s + 1] - 1, of which
+ * kv_lengths[s] (NULL: all) hold keys.  Offsets ascend; they are clamped to
+ * the tensors' rows, so wrong ones read and write nothing outside.  A query
+ * sees its sequence's keys, with `causal` key j of query i only where
+ * j <= i + keys - queries.  out [total_q, heads, dim] contiguous:
+ * softmax(scale q k^T) v; lse [heads, total_q] f32: log of the sum of
+ * exp(scale q k^T).  A query that sees no key, and a row of no sequence, gets
+ * out = 0 and lse = -inf.  Keys of no sequence and rows of k and v past
+ * kv_lengths may hold anything, NaN included; a non-finite v of a sequence may
+ * reach every query of that sequence, also those that do not see it.
+ *
+ * Backward: gradients of q, k and v (contiguous; zero where a row takes no
+ * part) from those of out and (nullable) lse.  Deterministic: the sums over
+ * queries, keys and the query heads of a key head have a fixed order.
+ * ---------------------------------------------------------------------- */
+int bfb_packed_attention_workspace_size(int64_t total_q, int64_t total_k, int64_t heads, int64_t kv_heads,
+                                        int64_t dim, int64_t seqs, int backward, size_t* bytes);
+
+int bfb_packed_attention(const void* q_dev, const void* k_dev, const void* v_dev, const int64_t* strides, int dtype,
+                         int64_t total_q, int64_t total_k, int64_t heads, int64_t kv_heads, int64_t dim,
+                         int64_t seqs, const int32_t* cu_q_dev, const int32_t* cu_k_dev,
+                         const int32_t* kv_lengths_dev, int causal, double scale, void* out_dev, float* lse_dev,
+                         void* workspace_dev, size_t workspace_bytes, void* stream);
+
+int bfb_packed_attention_backward(const void* out_grad_dev, const float* lse_grad_dev, const void* q_dev,
+                                  const void* k_dev, const void* v_dev, const int64_t* strides, const void* out_dev,
+                                  const float* lse_dev, int dtype, int64_t total_q, int64_t total_k, int64_t heads,
+                                  int64_t kv_heads, int64_t dim, int64_t seqs, const int32_t* cu_q_dev,
+                                  const int32_t* cu_k_dev, const int32_t* kv_lengths_dev, int causal, double scale,
+                                  void* q_grad_dev, void* k_grad_dev, void* v_grad_dev, void* workspace_dev,
+                                  size_t workspace_bytes, void* stream);
+
+/* Norm of each query and key head and its rotary position in one pass.
+ * q [tokens, heads, dim], k [tokens, kv_heads, dim] (f32 / f16 / bf16, row and
+ * head strides in elements, rows on 16 bytes), dim a multiple of 8 up to 256;
+ * outputs contiguous.  With a weight [dim] f32 (16-byte aligned, NULL: no
+ * norm) a head is x * rsqrt(mean(x^2) + eps) * weight; then its first
+ * `rotated` values are turned in pairs, (i, i + rotated / 2) or with
+ * `interleaved` (2 i, 2 i + 1): pair f by the angle positions[token, axis(f)] *
+ * inv_freq[f], axis(f) by `sections` (HOST, `axes` <= 8 counts that sum to
+ * rotated / 2: the first sections[0] pairs follow axis 0, and so on).
+ * rotated: a multiple of 16 (of 2 when interleaved).  Positions: element
+ * strides position_row and position_axis, position_type 0 = int32, 1 = int64,
+ * 2 = f32; inv_freq f32 or (inv_freq_f64) f64.  Angles are reduced in f64, so
+ * far positions are exact to f32.
+ *
+ * Backward: gradients of q and k (contiguous), and of the weights where given
+ * (f32 [dim], summed over tokens and heads in a fixed order). */
+int bfb_qk_norm_rotary(const void* q_dev, const void* k_dev, int64_t q_row, int64_t q_head, int64_t k_row,
+                       int64_t k_head, int dtype, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim,
+                       int64_t rotated, const void* positions_dev, int position_type, int64_t position_row,
+                       int64_t position_axis, const void* inv_freq_dev, int inv_freq_f64, int64_t axes,
+                       const int64_t* sections, const float* q_weight_dev, const float* k_weight_dev, double eps,
+                       int interleaved, void* q_out_dev, void* k_out_dev, void* stream);
+
+int bfb_qk_norm_rotary_backward_workspace_size(int64_t dim, size_t* bytes);
+
+int bfb_qk_norm_rotary_backward(const void* q_grad_dev, const void* k_grad_dev, const void* q_dev, const void* k_dev,
+                                int64_t q_row, int64_t q_head, int64_t k_row, int64_t k_head, int dtype,
+                                int64_t tokens, int64_t heads, int64_t kv_heads, int64_t dim, int64_t rotated,
+                                const void* positions_dev, int position_type, int64_t position_row,
+                                int64_t position_axis, const void* inv_freq_dev, int inv_freq_f64, int64_t axes,
+                                const int64_t* sections, const float* q_weight_dev, const float* k_weight_dev,
+                                double eps, int interleaved, void* q_input_grad_dev, void* k_input_grad_dev,
+                                float* q_weight_grad_dev, float* k_weight_grad_dev, void* workspace_dev,
+                                size_t workspace_bytes, void* stream);
+
+/* out = residual + keep * x / (1 - p) over n values (residual may be NULL).
+ * Value i is kept where word i % 4 of Philox4x32-10 at counter (i / 4,
+ * seed[1]) with key seed[0] is at least floor(p * 2^32), 0 <= p <= 1;
+ * seed: int64 [2] on the device.  The backward of x is the same call on the
+ * gradient without a residual. */
+int bfb_residual_dropout(const void* x_dev, const void* residual_dev, int dtype, int64_t n, const int64_t* seed_dev,
+                         double p, void* out_dev, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -8,7 +8,7 @@
 #include <algorithm>
 #include <cfloat>
 
-#include "common.cuh"
+#include "attention.cuh"
 
 namespace bfb {
 
@@ -17,21 +17,7 @@ BFB_DEBUG_READER(debug_violations_attention)
 
 namespace {
 
-struct Attn {
-  const void *q, *k, *v;
-  int64_t q_row, q_head, k_row, k_head, v_row, v_head;
-  int64_t total_q, total_k;
-  int heads, kv_heads, dim, seqs;
-  const int32_t *cu_q, *cu_k, *kv_lengths;
-  int causal;
-  float scale;
-  void* out;
-  float* lse;
-  // backward
-  const void* dout;
-  float* delta;
-  void *dq, *dk, *dv;
-};
+using Attn = attn::Args;
 
 struct Span {
   int64_t q0, k0;
@@ -86,40 +72,6 @@ __device__ __forceinline__ void row_store(T* p, int dim, const float (&v)[4]) {
 }
 __device__ __forceinline__ float dot4(const float (&a)[4], const float (&b)[4]) {
   return warp_sum(a[0] * b[0] + a[1] * b[1] + a[2] * b[2] + a[3] * b[3]);
-}
-
-// One warp per (query row, head).
-template <class T>
-__global__ void __launch_bounds__(128) forward_kernel(const __grid_constant__ Attn a) {
-  const int64_t unit = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (unit >= a.total_q * a.heads) return;
-  const int64_t r = unit / a.heads;
-  const int h = (int)(unit % a.heads), m = h / (a.heads / a.kv_heads);
-  const int seq = seq_of(a.cu_q, a.seqs, r);
-  float o[4] = {}, top = -INFINITY, sum = 0.f;
-  if (seq >= 0) {
-    const Span s = span_of(a, seq);
-    const int64_t i = r - s.q0;
-    const int64_t n = a.causal ? min((int64_t)s.lk, i + s.lk - s.lq + 1) : s.lk;
-    float q[4], x[4];
-    row_load<T>(static_cast<const T*>(a.q) + r * a.q_row + h * a.q_head, a.dim, q);
-    for (int64_t j = 0; j < n; ++j) {
-      row_load<T>(static_cast<const T*>(a.k) + (s.k0 + j) * a.k_row + m * a.k_head, a.dim, x);
-      const float score = dot4(q, x) * a.scale;
-      const float t = fmaxf(top, score);
-      const float keep = expf(top - t), p = expf(score - t);
-      top = t;
-      sum = sum * keep + p;
-      row_load<T>(static_cast<const T*>(a.v) + (s.k0 + j) * a.v_row + m * a.v_head, a.dim, x);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) o[c] = o[c] * keep + p * x[c];
-    }
-  }
-  const float inv = sum > 0.f ? 1.f / sum : 0.f;
-#pragma unroll
-  for (int c = 0; c < 4; ++c) o[c] *= inv;
-  row_store<T>(static_cast<T*>(a.out) + (r * a.heads + h) * a.dim, a.dim, o);
-  if ((threadIdx.x & 31) == 0) a.lse[h * a.total_q + r] = sum > 0.f ? top + logf(sum) : -INFINITY;
 }
 
 // delta = rowsum(dO o) - dlse, one warp per (row, head).
@@ -264,10 +216,13 @@ extern "C" int bfb_packed_attention(const void* q_dev, const void* k_dev, const 
   a.lse = lse_dev;
   BFB_TRY(check_args(a, dtype));
   if (total_q == 0) return BFB_OK;
-  auto kernel = dtype == BFB_F16 ? forward_kernel<__half> : forward_kernel<__nv_bfloat16>;
-  kernel<<<(unsigned)ceil_div(total_q * heads, 4), 128, 0, as_stream(stream)>>>(a);
-  BFB_CHECK_LAUNCH();
-  return BFB_OK;
+  return attn::forward_sm100(a, dtype, as_stream(stream));
+}
+
+extern "C" int bfb_attention_timeouts(uint64_t* count, int reset) {
+  if (!count) return BFB_ERR_INVALID_ARG;
+  *count = 0;
+  return attn::timeouts_forward(count, reset);
 }
 
 extern "C" int bfb_packed_attention_backward(

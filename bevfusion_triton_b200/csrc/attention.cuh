@@ -1,0 +1,109 @@
+// What the attention kernels share: the arguments of a call, the packed
+// sequences' rows, tensor maps.
+#pragma once
+
+#include "sm100.cuh"
+
+namespace bfb {
+namespace attn {
+
+struct Args {
+  const void *q, *k, *v;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head;
+  int64_t total_q, total_k;
+  int heads, kv_heads, dim, seqs;
+  const int32_t *cu_q, *cu_k, *kv_lengths;
+  int causal;
+  float scale;
+  void* out;
+  float* lse;
+  // backward
+  const void* dout;
+  float* delta;
+  void *dq, *dk, *dv;
+};
+
+constexpr int kTile = 128;  // rows of a tensor-core tile
+
+// Tiles of `rows` rows over packed sequences: the rows before the first and
+// after the last sequence count as two more, without keys, so that every row
+// of a tensor belongs to exactly one tile.  No more than this many tiles.
+inline int64_t tile_bound(int64_t total, int64_t seqs, int rows) { return total / rows + seqs + 2; }
+
+// Start of part i: part 0 holds the rows before sequence 0, part s + 1
+// sequence s, part seqs + 1 the rows behind the last.  Clamped to the tensor,
+// so offsets that are wrong cannot reach outside it.
+__device__ __forceinline__ int64_t part_start(const int32_t* cu, int seqs, int64_t total, int i) {
+  if (i == 0) return 0;
+  if (i > seqs + 1) return total;
+  return cu ? min(max((int64_t)cu[i - 1], (int64_t)0), total) : 0;
+}
+
+struct Tile {
+  int part;        // -1: no such tile
+  int64_t start;   // first row of the part
+  int rows;        // rows of the part
+  int index;       // tile within the part
+};
+
+// The item-th tile, found by one warp (all lanes take part and all get it).
+__device__ __forceinline__ Tile find_tile(const int32_t* cu, int seqs, int64_t total, int rows, int64_t item) {
+  const int lane = threadIdx.x & 31;
+  int64_t before = 0;
+  for (int base = 0; base < seqs + 2; base += 32) {
+    const int part = base + lane;
+    int64_t start = 0, n = 0;
+    if (part < seqs + 2) {
+      start = part_start(cu, seqs, total, part);
+      n = max(part_start(cu, seqs, total, part + 1) - start, (int64_t)0);
+    }
+    const int64_t tiles = (n + rows - 1) / rows;
+    int64_t upto = tiles;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, item < before + upto);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      Tile t;
+      t.part = base + src;
+      t.start = __shfl_sync(0xffffffffu, start, src);
+      t.rows = (int)__shfl_sync(0xffffffffu, n, src);
+      t.index = (int)(item - before - __shfl_sync(0xffffffffu, upto - tiles, src));
+      return t;
+    }
+    before += __shfl_sync(0xffffffffu, upto, 31);
+  }
+  return {-1, 0, 0, 0};
+}
+
+// Rows of part `part` in the other tensor of the pair (none for the parts
+// that are no sequence).
+__device__ __forceinline__ void other_rows(const int32_t* cu, int seqs, int64_t total, int part, int64_t& start,
+                                           int& rows) {
+  start = 0;
+  rows = 0;
+  if (part < 1 || part > seqs) return;
+  start = part_start(cu, seqs, total, part);
+  rows = (int)max(part_start(cu, seqs, total, part + 1) - start, (int64_t)0);
+}
+
+__device__ __forceinline__ int used_keys(const int32_t* kv_lengths, int part, int rows) {
+  return kv_lengths && rows > 0 ? min(max(kv_lengths[part - 1], 0), rows) : rows;
+}
+
+// Tensor map of [rows, heads, dim] 16-bit values whose box is 128 rows of 64
+// values of one head, in the 128-byte swizzle; values past dim and rows past
+// the tensor read as zeros.
+int make_map(CUtensorMap* map, const void* base, int dtype, int64_t rows, int heads, int dim, int64_t row_stride,
+             int64_t head_stride);
+
+int forward_sm100(const Args& a, int dtype, cudaStream_t stream);
+int backward_sm100(const Args& a, int dtype, cudaStream_t stream);
+int timeouts_forward(uint64_t* count, int reset);
+int timeouts_backward(uint64_t* count, int reset);
+
+}  // namespace attn
+}  // namespace bfb

@@ -517,6 +517,10 @@ int bfb_packed_attention_backward(const void* out_grad_dev, const float* lse_gra
                                   void* q_grad_dev, void* k_grad_dev, void* v_grad_dev, void* workspace_dev,
                                   size_t workspace_bytes, void* stream);
 
+/* Number of bounded waits in the attention kernels that gave up (0 in a
+ * correct run); reset = 1 clears it.  Synchronous. */
+int bfb_attention_timeouts(uint64_t* count, int reset);
+
 /* Norm of each query and key head and its rotary position in one pass.
  * q [tokens, heads, dim], k [tokens, kv_heads, dim] (f32 / f16 / bf16, row and
  * head strides in elements, rows on 16 bytes), dim a multiple of 8 up to 256;

@@ -1,17 +1,28 @@
 """packed_attention, qk_norm_rotary, residual_dropout and SparseSelfAttention
 on the GPU against the 64-bit oracle, within tolerances counted from the
 roundings (tests/attention_oracle.py)."""
+import ctypes
 import math
 
 import numpy as np
 import pytest
 import torch
 
+from bevfusion_triton_b200 import load_native
 from bevfusion_triton_b200.ops.spconv import (SparseConvTensor, SparseSelfAttention, SparseSequential,
                                               packed_attention, qk_norm_rotary, residual_dropout)
 from tests import attention_oracle as oracle
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def no_wait_gave_up():
+    yield
+    if torch.cuda.is_available():
+        count = ctypes.c_uint64()
+        assert load_native().bfb_attention_timeouts(ctypes.byref(count), 1) == 0 and count.value == 0
+
 
 F16, BF16, F32 = torch.float16, torch.bfloat16, torch.float32
 

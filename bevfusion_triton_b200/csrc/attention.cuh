@@ -19,7 +19,8 @@ struct Args {
   float* lse;
   // backward
   const void* dout;
-  float* delta;
+  const float* dlse;     // may be NULL
+  float *lse2, *delta;   // workspace, [heads, total_q] each
   void *dq, *dk, *dv;
 };
 

@@ -1,0 +1,624 @@
+// Packed attention, backward, on the tensor cores.  With c = scale log2(e),
+//   P = exp2(c S - lse2),  dS = P (scale dP - scale delta)
+// one kernel owns key tiles and sums dK and dV over the query tiles and the
+// query heads of its key head, another owns query tiles and sums dQ over the
+// key tiles.  That computes S and dP twice (seven products for the five that
+// one kernel with dQ in atomics would need), but every sum has a fixed order,
+// no fp32 copy of dQ goes through memory, and nothing has to be cleared first.
+//
+// Both keep their sums in tensor memory over the whole walk.  dS (and P for
+// dV) are rounded to 16 bits and stay in tensor memory, over the scores they
+// came from, as the next product's first operand; each 128 x 128 step is
+// worked by two warpgroups, one per 64 columns, with 64 values per thread.
+// dS carries the scale before it is rounded: in fp16 it then overflows only
+// where the gradient itself is near to.
+#include <algorithm>
+
+#include "attention.cuh"
+
+namespace bfb {
+namespace attn {
+
+namespace {
+
+using namespace sm100;
+
+__device__ unsigned long long g_timeouts = 0ull;
+
+constexpr int kThreads = 384;  // warps 0-7 work on the scores, 8 issues products, 9 loads
+constexpr int kHalf = kTile / 2;
+constexpr float kLog2e = 1.4426950408889634f;
+
+template <int DP>
+struct Layout {
+  static constexpr int kTileBytes = kTile * DP * 2;
+  static constexpr int kPanel = kTile * 128;
+  static constexpr int kTiles = 7;  // two resident tiles, three of the first ring, two of the second
+};
+
+// The walked tensors come through two rings: the first (queries or keys) is
+// read by the scores and again by the last product of its step, so it needs a
+// stage more than the second to be loaded in time.
+constexpr int kFirst = 3, kSecond = 2;
+
+struct Shared {
+  uint64_t own_full, a_full[kFirst], a_empty[kFirst], b_full[kSecond], b_empty[kSecond];
+  uint64_t s_full, dp_full, p_ready, ds_ready, done, tail;
+  uint32_t tmem;
+  int part, tile, lq, lk, room;
+  int64_t q0, k0;
+  float lse2[kFirst][kTile], delta[kSecond][kTile];
+};
+
+template <int DP>
+constexpr size_t smem_bytes() { return (size_t)Layout<DP>::kTiles * Layout<DP>::kTileBytes + sizeof(Shared); }
+static_assert(smem_bytes<128>() <= 227 * 1024, "a block's shared memory");
+
+// K steps of 16 of a 16-bit operand that two warpgroups wrote as 2 x 64
+// columns: the second half starts 64 columns of tensor memory later.
+__device__ __forceinline__ constexpr uint32_t half_step(int c) { return (c >> 2) * kHalf + (c & 3) * 8; }
+
+// Clears the rows from `valid` on of a tile in shared memory, by one warp.
+// Rows behind a sequence meet zeros of P and dS in the products, but 0 * NaN
+// is not 0.
+template <int DP>
+__device__ __forceinline__ void clear_rows(uint8_t* tile, int valid) {
+  for (int c = 0; c < DP / 64; ++c)
+    for (int b = valid * 8 + (threadIdx.x & 31); b < kTile * 8; b += 32)
+      reinterpret_cast<uint4*>(tile + c * Layout<DP>::kPanel)[b] = make_uint4(0, 0, 0, 0);
+}
+
+template <int DP>
+__device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* map, int head, int64_t row, uint64_t* bar) {
+#pragma unroll
+  for (int c = 0; c < DP / 64; ++c) tma_load(dst + c * Layout<DP>::kPanel, map, 64 * c, head, (int)row, bar);
+}
+
+// dst += A B over 128 rows of B (A in tensor memory, B's rows along K).
+template <int DP, bool kBf16>
+__device__ __forceinline__ void product_rows(uint32_t dst, uint32_t a, uint32_t b, bool first) {
+#pragma unroll
+  for (int c = 0; c < kTile / 16; ++c)
+    mma_ts(dst, a + half_step(c), tile_desc(b + c * 2048, Layout<DP>::kPanel), mma_desc(kBf16, DP, true),
+           !first || c > 0);
+}
+// dst = A B^T over the columns of two tiles.
+template <int DP, bool kBf16>
+__device__ __forceinline__ void product_cols(uint32_t dst, uint32_t a, uint32_t b) {
+#pragma unroll
+  for (int c = 0; c < DP / 16; ++c) {
+    const uint32_t off = (c / 4) * Layout<DP>::kPanel + (c % 4) * 32;
+    mma_ss(dst, tile_desc(a + off, 16), tile_desc(b + off, 16), mma_desc(kBf16, kTile, false), c > 0);
+  }
+}
+
+// `cols` fp32 columns of a 128-row sum from tensor memory, as 16-bit values
+// [col0, col0 + cols) of a row of [rows, heads, dim].
+template <class T>
+__device__ __forceinline__ void write_row(uint32_t from, T* out, int col0, int cols, int dim, bool live, bool zero) {
+  for (int b = 0; b < cols; b += 32) {
+    uint32_t o[32];
+    tmem_ld32(from + b, o);
+    tmem_ld_wait32(o);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int col = col0 + b + 8 * e;
+      if (!live || col >= dim) continue;
+      uint4 w = make_uint4(0, 0, 0, 0);
+      uint32_t* ww = reinterpret_cast<uint32_t*>(&w);
+      if (!zero) {
+#pragma unroll
+        for (int f = 0; f < 4; ++f)
+          ww[f] = pack2<T>(__uint_as_float(o[8 * e + 2 * f]), __uint_as_float(o[8 * e + 2 * f + 1]));
+      }
+      *reinterpret_cast<uint4*>(out + col) = w;
+    }
+  }
+}
+
+// Finds the block's tile (of keys, or of queries) and its sequence, sets up
+// the barriers; false if there is no such tile.
+template <bool kKeys>
+__device__ __forceinline__ bool setup(Shared& s, const Args& a, int64_t item) {
+  if (threadIdx.x < 32) {
+    const Tile t = kKeys ? find_tile(a.cu_k, a.seqs, a.total_k, kTile, item)
+                         : find_tile(a.cu_q, a.seqs, a.total_q, kTile, item);
+    if (threadIdx.x == 0) {
+      s.part = t.part;
+      if (t.part >= 0) {
+        int64_t start;
+        int rows;
+        if (kKeys) {
+          other_rows(a.cu_q, a.seqs, a.total_q, t.part, start, rows);
+          s.k0 = t.start;
+          s.room = t.rows;
+          s.q0 = start;
+          s.lq = rows;
+          s.lk = t.part >= 1 && t.part <= a.seqs ? used_keys(a.kv_lengths, t.part, t.rows) : 0;
+          s.tile = t.index;
+        } else {
+          other_rows(a.cu_k, a.seqs, a.total_k, t.part, start, rows);
+          s.q0 = t.start;
+          s.lq = t.rows;
+          s.k0 = start;
+          s.lk = used_keys(a.kv_lengths, t.part, rows);
+          // causal: the last tiles, which see the most keys, start first
+          s.tile = (t.rows + kTile - 1) / kTile - 1 - t.index;
+        }
+      }
+      bar_init(&s.own_full, 1);
+      for (int i = 0; i < kFirst; ++i) {
+        bar_init(&s.a_full[i], 2);
+        bar_init(&s.a_empty[i], 1);
+      }
+      for (int i = 0; i < kSecond; ++i) {
+        bar_init(&s.b_full[i], 2);
+        bar_init(&s.b_empty[i], 1);
+      }
+      bar_init(&s.s_full, 1);
+      bar_init(&s.dp_full, 1);
+      bar_init(&s.p_ready, 2 * kTile);
+      bar_init(&s.ds_ready, 2 * kTile);
+      bar_init(&s.done, 1);
+      bar_init(&s.tail, 1);
+      fence_bar_init();
+    }
+  }
+  __syncthreads();
+  return s.part >= 0;
+}
+
+__device__ __forceinline__ uint32_t tmem_start(Shared& s, int warp) {
+  if (warp == 8) tmem_alloc(&s.tmem, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  return s.tmem;
+}
+__device__ __forceinline__ void tmem_end(Shared& s, int warp) {
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 8) {
+    tc_fence_after();
+    tmem_free(s.tmem, 512);
+  }
+}
+
+// One warp's load of a ring's stage: waits for the stage, fetches `tile`'s
+// rows by TMA, has `extra` fill what goes with them, clears the rows from
+// `valid` on (kClear), and signals `full` (two arrivals).
+template <int DP, bool kClear, class F>
+__device__ __forceinline__ bool load_stage(uint8_t* dst, const CUtensorMap* map, int head, int64_t row, int valid,
+                                           uint64_t* full, uint64_t* empty, uint32_t parity, uint64_t* tail,
+                                           uint32_t& tails, F extra) {
+  const int lane = threadIdx.x & 31;
+  bool ok = true;
+  if (lane == 0) ok = bar_wait(empty, parity ^ 1, &g_timeouts);
+  if (!__shfl_sync(0xffffffffu, ok, 0)) return false;
+  const bool clear = kClear && valid < kTile;
+  if (lane == 0) {
+    uint64_t* bar = clear ? tail : full;
+    bar_expect(bar, Layout<DP>::kTileBytes);
+    load_tile<DP>(dst, map, head, row, bar);
+  }
+  extra();
+  if (clear) {
+    ok = bar_wait(tail, tails & 1, &g_timeouts);
+    ++tails;
+    if (!__all_sync(0xffffffffu, ok)) return false;
+    clear_rows<DP>(dst, valid);
+    fence_async_smem();
+  }
+  __syncwarp();
+  if (lane == 0) {
+    bar_arrive(full);
+    if (clear) bar_arrive(full);
+  }
+  return true;
+}
+
+// A loader that gave up leaves only when what it has asked for has landed:
+// the resident tiles, the last loads of both rings (a_loads and b_loads
+// issued), and one waiting to be cleared.
+__device__ __forceinline__ void drain_loads(Shared& s, int a_loads, int b_loads, uint32_t tails) {
+  bar_wait(&s.own_full, 0, &g_timeouts);
+  for (int i = max(0, a_loads - kFirst); i < a_loads; ++i)
+    bar_wait(&s.a_full[i % kFirst], (i / kFirst) & 1, &g_timeouts);
+  for (int i = max(0, b_loads - kSecond); i < b_loads; ++i)
+    bar_wait(&s.b_full[i % kSecond], (i / kSecond) & 1, &g_timeouts);
+  if (tails > 0) bar_wait(&s.tail, (tails - 1) & 1, &g_timeouts);
+}
+
+// ------------------------------------------------------------------ dK and dV
+// S^T = K Q^T, dP^T = V dO^T, dV += P^T dO, dK += dS^T Q: a thread owns one
+// key row.  While the warpgroups form P the tensor core makes dP, while they
+// form dS it adds to dV and makes the next S, and dK with the next dP after
+// that: one buffer of each is enough, 128 + 128 + 2 DP columns.
+template <class T, int DP>
+__global__ void __launch_bounds__(kThreads, 1)
+    dkv_kernel(const __grid_constant__ Args a, const __grid_constant__ CUtensorMap q_map,
+               const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+               const __grid_constant__ CUtensorMap g_map) {
+  using L = Layout<DP>;
+  constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  extern __shared__ __align__(1024) uint8_t tiles[];
+  Shared& s = *reinterpret_cast<Shared*>(tiles + L::kTiles * L::kTileBytes);
+  uint8_t *sk = tiles, *sv = sk + L::kTileBytes, *sq = sv + L::kTileBytes, *sg = sq + kFirst * L::kTileBytes;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int m = blockIdx.x % a.kv_heads, group = a.heads / a.kv_heads;
+  if (!setup<true>(s, a, blockIdx.x / a.kv_heads)) return;
+  const uint32_t tmem = tmem_start(s, warp);
+  const uint32_t ts = tmem, tdp = tmem + kTile, tdv = tmem + 2 * kTile, tdk = tdv + DP;
+  const int lq = s.lq, lk = s.lk, j0 = s.tile * kTile, shift = lk - lq;
+  // query tiles that see any of these keys: from the one with the first row i that has i + shift >= j0
+  const int first = a.causal ? max(0, j0 - shift) / kTile : 0;
+  const int per_head = j0 < lk ? max(0, (lq + kTile - 1) / kTile - first) : 0;
+  const int n = per_head * group;
+
+  if (warp < 8) {
+    regs_grow<208>();
+    const int wg = warp >> 2, row = threadIdx.x & (kTile - 1), j = j0 + row;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, mine = lanes + wg * kHalf;
+    const float c = a.scale * kLog2e;
+    bool ok = true;
+    int tile = 0;
+    for (int i = 0; i < n; ++i) {
+      const int sa = i % kFirst, sb = i % kSecond;
+      if (!(ok = bar_wait(&s.a_full[sa], (i / kFirst) & 1, &g_timeouts) && bar_wait(&s.s_full, i & 1, &g_timeouts)))
+        break;
+      tc_fence_after();
+      uint32_t x[kHalf];
+      tmem_ld32(ts + mine, x);
+      tmem_ld32(ts + mine + 32, x + 32);
+      // the half's first query, and the first of its columns from which key row j is seen
+      const int q = (first + tile) * kTile + wg * kHalf;
+      if (++tile == per_head) tile = 0;
+      const int from = j - shift - q;
+      const bool masked = a.causal && j0 + kTile - 1 - shift - q > 0;
+      const float* lse2 = s.lse2[sa] + wg * kHalf;
+      const float* delta = s.delta[sb] + wg * kHalf;
+      tmem_ld_wait32(x);
+      tmem_ld_wait32(x + 32);
+      float p[kHalf];
+#pragma unroll
+      for (int e = 0; e < kHalf; ++e) {
+        p[e] = exp2_approx(fmaf(__uint_as_float(x[e]), c, -lse2[e]));
+        if (masked && e < from) p[e] = 0.f;
+      }
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        uint32_t w[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) w[e] = pack2<T>(p[32 * b + 2 * e], p[32 * b + 2 * e + 1]);
+        tmem_st16(ts + mine + 16 * b, w);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      bar_arrive(&s.p_ready);
+      if (!(ok = bar_wait(&s.b_full[sb], (i / kSecond) & 1, &g_timeouts) && bar_wait(&s.dp_full, i & 1, &g_timeouts)))
+        break;
+      tc_fence_after();
+      tmem_ld32(tdp + mine, x);
+      tmem_ld32(tdp + mine + 32, x + 32);
+      tmem_ld_wait32(x);
+      tmem_ld_wait32(x + 32);
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        uint32_t w[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int at = 32 * b + 2 * e;
+          float u = p[at] * fmaf(__uint_as_float(x[at]), a.scale, -delta[at]);
+          float v = p[at + 1] * fmaf(__uint_as_float(x[at + 1]), a.scale, -delta[at + 1]);
+          if (masked) {
+            if (at < from) u = 0.f;
+            if (at + 1 < from) v = 0.f;
+          }
+          w[e] = pack2<T>(u, v);
+        }
+        tmem_st16(tdp + mine + 16 * b, w);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      bar_arrive(&s.ds_ready);
+    }
+    if (ok && (n == 0 || bar_wait(&s.done, 0, &g_timeouts))) {
+      tc_fence_after();
+      T* out = static_cast<T*>(wg ? a.dk : a.dv) + ((s.k0 + j) * a.kv_heads + m) * a.dim;
+      write_row<T>((wg ? tdk : tdv) + lanes, out, 0, DP, a.dim, j < s.room, n == 0 || j >= lk);
+    }
+  } else {
+    regs_shrink<88>();
+    if (warp == 8 && lane == 0 && n > 0) {
+      const uint32_t ka = smem_u32(sk), va = smem_u32(sv);
+      auto q_at = [&](int i) { return smem_u32(sq + (i % kFirst) * L::kTileBytes); };
+      auto g_at = [&](int i) { return smem_u32(sg + (i % kSecond) * L::kTileBytes); };
+      auto q_full = [&](int i) { return bar_wait(&s.a_full[i % kFirst], (i / kFirst) & 1, &g_timeouts); };
+      auto g_full = [&](int i) { return bar_wait(&s.b_full[i % kSecond], (i / kSecond) & 1, &g_timeouts); };
+      bool ok = bar_wait(&s.own_full, 0, &g_timeouts) && q_full(0) && g_full(0);
+      if (ok) {
+        tc_fence_after();
+        product_cols<DP, kBf16>(ts, ka, q_at(0));
+        mma_commit(&s.s_full);
+        product_cols<DP, kBf16>(tdp, va, g_at(0));
+        mma_commit(&s.dp_full);
+      }
+      for (int i = 0; i < n && ok; ++i) {
+        const bool more = i + 1 < n;
+        if (!(ok = bar_wait(&s.p_ready, i & 1, &g_timeouts))) break;
+        tc_fence_after();
+        product_rows<DP, kBf16>(tdv, ts, g_at(i), i == 0);
+        if (more) {
+          if (!(ok = q_full(i + 1))) break;
+          product_cols<DP, kBf16>(ts, ka, q_at(i + 1));
+          mma_commit(&s.s_full);
+        }
+        if (!(ok = bar_wait(&s.ds_ready, i & 1, &g_timeouts))) break;
+        tc_fence_after();
+        product_rows<DP, kBf16>(tdk, tdp, q_at(i), i == 0);
+        // both: the threads are done with lse2 and delta, too
+        mma_commit(&s.a_empty[i % kFirst]);
+        mma_commit(&s.b_empty[i % kSecond]);
+        if (more) {
+          if (!(ok = g_full(i + 1))) break;
+          product_cols<DP, kBf16>(tdp, va, g_at(i + 1));
+          mma_commit(&s.dp_full);
+        }
+      }
+      mma_commit(&s.done);
+      bar_wait(&s.done, 0, &g_timeouts);  // nothing leaves before its products are done
+    } else if (warp == 9 && n > 0) {
+      if (lane == 0) {
+        bar_expect(&s.own_full, 2 * L::kTileBytes);
+        load_tile<DP>(sk, &k_map, m, s.k0 + j0, &s.own_full);
+        load_tile<DP>(sv, &v_map, m, s.k0 + j0, &s.own_full);
+      }
+      uint32_t tails = 0;
+      int i = 0, a_loads = 0, tile = 0, h = m * group;
+      for (; i < n; ++i) {
+        const int q = (first + tile) * kTile, valid = lq - q, sa = i % kFirst, sb = i % kSecond;
+        const int64_t at = (int64_t)h * a.total_q + s.q0 + q;
+        // rows past the sequence: P = exp2(-inf) = 0
+        if (!load_stage<DP, true>(sq + sa * L::kTileBytes, &q_map, h, s.q0 + q, valid, &s.a_full[sa], &s.a_empty[sa],
+                                  (i / kFirst) & 1, &s.tail, tails, [&] {
+                                    for (int r = lane; r < kTile; r += 32)
+                                      s.lse2[sa][r] = r < valid ? a.lse2[at + r] : INFINITY;
+                                  }))
+          break;
+        ++a_loads;
+        if (!load_stage<DP, true>(sg + sb * L::kTileBytes, &g_map, h, s.q0 + q, valid, &s.b_full[sb], &s.b_empty[sb],
+                                  (i / kSecond) & 1, &s.tail, tails, [&] {
+                                    for (int r = lane; r < kTile; r += 32)
+                                      s.delta[sb][r] = r < valid ? a.delta[at + r] : 0.f;
+                                  }))
+          break;
+        if (++tile == per_head) {
+          tile = 0;
+          ++h;
+        }
+      }
+      if (lane == 0 && i < n) drain_loads(s, a_loads, i, tails);
+    }
+  }
+  tmem_end(s, warp);
+}
+
+// ------------------------------------------------------------------------- dQ
+// S = Q K^T, dP = dO V^T, dQ += dS K: a thread owns one query row.  P only
+// lives in registers, so S's columns are free for the next one as soon as
+// they have been read.
+template <class T, int DP>
+__global__ void __launch_bounds__(kThreads, 1)
+    dq_kernel(const __grid_constant__ Args a, const __grid_constant__ CUtensorMap q_map,
+              const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+              const __grid_constant__ CUtensorMap g_map) {
+  using L = Layout<DP>;
+  constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+  extern __shared__ __align__(1024) uint8_t tiles[];
+  Shared& s = *reinterpret_cast<Shared*>(tiles + L::kTiles * L::kTileBytes);
+  uint8_t *sq = tiles, *sg = sq + L::kTileBytes, *sk = sg + L::kTileBytes, *sv = sk + kFirst * L::kTileBytes;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int h = blockIdx.x % a.heads, m = h / (a.heads / a.kv_heads);
+  if (!setup<false>(s, a, blockIdx.x / a.heads)) return;
+  const uint32_t tmem = tmem_start(s, warp);
+  const uint32_t ts = tmem, tdp = tmem + kTile, tdq = tmem + 2 * kTile;
+  const int lq = s.lq, lk = s.lk, i0 = s.tile * kTile, shift = lk - lq;
+  auto seen = [&](int i) { return a.causal ? max(0, min(lk, i + shift + 1)) : lk; };
+  const int n = (seen(min(lq, i0 + kTile) - 1) + kTile - 1) / kTile;
+
+  if (warp < 8) {
+    regs_grow<208>();
+    const int wg = warp >> 2, row = threadIdx.x & (kTile - 1), i = i0 + row;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, mine = lanes + wg * kHalf;
+    const float c = a.scale * kLog2e;
+    const int64_t at = (int64_t)h * a.total_q + s.q0 + i;
+    const float lse2 = i < lq ? a.lse2[at] : INFINITY, delta = i < lq ? a.delta[at] : 0.f;
+    const int sees = seen(i), warp_sees = seen(i - lane);
+    bool ok = true;
+    for (int j = 0; j < n; ++j) {
+      if (!(ok = bar_wait(&s.s_full, j & 1, &g_timeouts))) break;
+      tc_fence_after();
+      uint32_t x[kHalf];
+      tmem_ld32(ts + mine, x);
+      tmem_ld32(ts + mine + 32, x + 32);
+      tmem_ld_wait32(x);
+      tmem_ld_wait32(x + 32);
+      tc_fence_before();
+      bar_arrive(&s.p_ready);  // S is read
+      const int limit = sees - j * kTile - wg * kHalf;
+      const bool masked = warp_sees < j * kTile + wg * kHalf + kHalf;
+      float p[kHalf];
+#pragma unroll
+      for (int e = 0; e < kHalf; ++e) p[e] = exp2_approx(fmaf(__uint_as_float(x[e]), c, -lse2));
+      if (!(ok = bar_wait(&s.dp_full, j & 1, &g_timeouts))) break;
+      tc_fence_after();
+      tmem_ld32(tdp + mine, x);
+      tmem_ld32(tdp + mine + 32, x + 32);
+      tmem_ld_wait32(x);
+      tmem_ld_wait32(x + 32);
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        uint32_t w[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int col = 32 * b + 2 * e;
+          float u = p[col] * fmaf(__uint_as_float(x[col]), a.scale, -delta);
+          float v = p[col + 1] * fmaf(__uint_as_float(x[col + 1]), a.scale, -delta);
+          if (masked) {
+            if (col >= limit) u = 0.f;
+            if (col + 1 >= limit) v = 0.f;
+          }
+          w[e] = pack2<T>(u, v);
+        }
+        tmem_st16(tdp + mine + 16 * b, w);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      bar_arrive(&s.ds_ready);
+    }
+    if (ok && (n == 0 || bar_wait(&s.done, 0, &g_timeouts))) {
+      tc_fence_after();
+      T* out = static_cast<T*>(a.dq) + ((s.q0 + i) * a.heads + h) * a.dim;
+      write_row<T>(tdq + lanes + wg * (DP / 2), out, wg * (DP / 2), DP / 2, a.dim, i < lq, n == 0);
+    }
+  } else {
+    regs_shrink<88>();
+    if (warp == 8 && lane == 0 && n > 0) {
+      const uint32_t qa = smem_u32(sq), ga = smem_u32(sg);
+      auto k_at = [&](int j) { return smem_u32(sk + (j % kFirst) * L::kTileBytes); };
+      auto v_at = [&](int j) { return smem_u32(sv + (j % kSecond) * L::kTileBytes); };
+      auto k_full = [&](int j) { return bar_wait(&s.a_full[j % kFirst], (j / kFirst) & 1, &g_timeouts); };
+      auto v_full = [&](int j) { return bar_wait(&s.b_full[j % kSecond], (j / kSecond) & 1, &g_timeouts); };
+      bool ok = bar_wait(&s.own_full, 0, &g_timeouts) && k_full(0) && v_full(0);
+      if (ok) {
+        tc_fence_after();
+        product_cols<DP, kBf16>(ts, qa, k_at(0));
+        mma_commit(&s.s_full);
+        product_cols<DP, kBf16>(tdp, ga, v_at(0));
+        mma_commit(&s.dp_full);
+        mma_commit(&s.b_empty[0]);
+      }
+      for (int j = 0; j < n && ok; ++j) {
+        const bool more = j + 1 < n;
+        if (!(ok = bar_wait(&s.p_ready, j & 1, &g_timeouts))) break;
+        tc_fence_after();
+        if (more) {
+          if (!(ok = k_full(j + 1))) break;
+          product_cols<DP, kBf16>(ts, qa, k_at(j + 1));
+          mma_commit(&s.s_full);
+        }
+        if (!(ok = bar_wait(&s.ds_ready, j & 1, &g_timeouts))) break;
+        tc_fence_after();
+        product_rows<DP, kBf16>(tdq, tdp, k_at(j), j == 0);
+        mma_commit(&s.a_empty[j % kFirst]);
+        if (more) {
+          if (!(ok = v_full(j + 1))) break;
+          product_cols<DP, kBf16>(tdp, ga, v_at(j + 1));
+          mma_commit(&s.dp_full);
+          mma_commit(&s.b_empty[(j + 1) % kSecond]);
+        }
+      }
+      mma_commit(&s.done);
+      bar_wait(&s.done, 0, &g_timeouts);
+    } else if (warp == 9 && n > 0) {
+      if (lane == 0) {
+        bar_expect(&s.own_full, 2 * L::kTileBytes);
+        load_tile<DP>(sq, &q_map, h, s.q0 + i0, &s.own_full);
+        load_tile<DP>(sg, &g_map, h, s.q0 + i0, &s.own_full);
+      }
+      uint32_t tails = 0;
+      int j = 0, a_loads = 0;
+      for (; j < n; ++j) {
+        const int valid = lk - j * kTile, sa = j % kFirst, sb = j % kSecond;
+        const int64_t k = s.k0 + (int64_t)j * kTile;
+        if (!load_stage<DP, true>(sk + sa * L::kTileBytes, &k_map, m, k, valid, &s.a_full[sa], &s.a_empty[sa],
+                                  (j / kFirst) & 1, &s.tail, tails, [] {}))
+          break;
+        ++a_loads;
+        if (!load_stage<DP, false>(sv + sb * L::kTileBytes, &v_map, m, k, valid, &s.b_full[sb], &s.b_empty[sb],
+                                   (j / kSecond) & 1, &s.tail, tails, [] {}))
+          break;
+      }
+      if (lane == 0 && j < n) drain_loads(s, a_loads, j, tails);
+    }
+  }
+  tmem_end(s, warp);
+}
+
+// What both kernels read for each query and head: lse2 = log2(e) lse, +inf
+// where no key is seen (so that P = 0), and delta = scale (rowsum(dO o) - dlse).
+// A group of lanes takes a row, 16 bytes each.
+template <class T>
+__global__ void __launch_bounds__(256) rows_kernel(const __grid_constant__ Args a, int lanes) {
+  const int64_t unit = ((int64_t)blockIdx.x * 256 + threadIdx.x) / lanes;  // row * heads + head
+  const int lane = threadIdx.x & (lanes - 1);
+  const bool live = unit < a.total_q * a.heads;
+  float d = 0.f;
+  if (live && lane * 8 < a.dim) {
+    const uint4 x = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.out) + unit * a.dim + lane * 8);
+    const uint4 y = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.dout) + unit * a.dim + lane * 8);
+    const T *u = reinterpret_cast<const T*>(&x), *v = reinterpret_cast<const T*>(&y);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) d += to_f32<T>(u[e]) * to_f32<T>(v[e]);
+  }
+  for (int o = lanes >> 1; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+  if (!live || lane > 0) return;
+  const int64_t r = unit / a.heads, at = (unit - r * a.heads) * a.total_q + r;
+  const float lse = a.lse[at];
+  a.lse2[at] = lse == -INFINITY ? INFINITY : lse * kLog2e;
+  a.delta[at] = a.scale * (d - (a.dlse ? a.dlse[at] : 0.f));
+}
+
+template <class T, int DP>
+int launch(const Args& a, int dtype, cudaStream_t stream) {
+  constexpr int kBytes = (int)smem_bytes<DP>();
+  // first: it makes the device's context current on this thread, which the tensor maps need
+  BFB_CUDA(cudaFuncSetAttribute(dkv_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes));
+  BFB_CUDA(cudaFuncSetAttribute(dq_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize, kBytes));
+  CUtensorMap q, k, v, g;
+  const void* any = a.total_q ? a.q : a.k;  // an address for the maps of tensors without rows: never loaded
+  BFB_TRY(make_map(&q, a.total_q ? a.q : any, dtype, a.total_q, a.heads, a.dim, a.q_row, a.q_head));
+  BFB_TRY(make_map(&g, a.total_q ? a.dout : any, dtype, a.total_q, a.heads, a.dim, (int64_t)a.heads * a.dim, a.dim));
+  BFB_TRY(make_map(&k, a.total_k ? a.k : any, dtype, a.total_k, a.kv_heads, a.dim, a.k_row, a.k_head));
+  BFB_TRY(make_map(&v, a.total_k ? a.v : any, dtype, a.total_k, a.kv_heads, a.dim, a.v_row, a.v_head));
+  const int64_t q_blocks = tile_bound(a.total_q, a.seqs, kTile) * a.heads;
+  const int64_t k_blocks = tile_bound(a.total_k, a.seqs, kTile) * a.kv_heads;
+  int lanes = 1;
+  while (lanes * 8 < a.dim) lanes <<= 1;
+  const int64_t row_blocks = ceil_div(a.total_q * a.heads * lanes, 256);
+  if (std::max(std::max(q_blocks, k_blocks), row_blocks) > 0x7fffffff) return BFB_ERR_TOO_LARGE;
+  if (a.total_q > 0) {
+    rows_kernel<T><<<(unsigned)row_blocks, 256, 0, stream>>>(a, lanes);
+    BFB_CHECK_LAUNCH();
+  }
+  if (a.total_k > 0) {
+    dkv_kernel<T, DP><<<(unsigned)k_blocks, kThreads, kBytes, stream>>>(a, q, k, v, g);
+    BFB_CHECK_LAUNCH();
+  }
+  if (a.total_q > 0) {
+    dq_kernel<T, DP><<<(unsigned)q_blocks, kThreads, kBytes, stream>>>(a, q, k, v, g);
+    BFB_CHECK_LAUNCH();
+  }
+  return BFB_OK;
+}
+
+}  // namespace
+
+int backward_sm100(const Args& a, int dtype, cudaStream_t stream) {
+  if (dtype == BFB_F16) return a.dim <= 64 ? launch<__half, 64>(a, dtype, stream) : launch<__half, 128>(a, dtype, stream);
+  return a.dim <= 64 ? launch<__nv_bfloat16, 64>(a, dtype, stream) : launch<__nv_bfloat16, 128>(a, dtype, stream);
+}
+
+int timeouts_backward(uint64_t* count, int reset) {
+  unsigned long long x = 0ull;
+  BFB_CUDA(cudaMemcpyFromSymbol(&x, g_timeouts, sizeof(x)));
+  if (reset) {
+    const unsigned long long z = 0ull;
+    BFB_CUDA(cudaMemcpyToSymbol(g_timeouts, &z, sizeof(z)));
+  }
+  *count += x;
+  return BFB_OK;
+}
+
+}  // namespace attn
+}  // namespace bfb

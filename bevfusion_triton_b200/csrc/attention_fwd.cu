@@ -348,6 +348,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 template <class T, int DP>
 int launch(const Args& a, int dtype, cudaStream_t stream) {
+  // first: it makes the device's context current on this thread, which the tensor maps need
+  BFB_CUDA(cudaFuncSetAttribute(forward_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                Layout<DP>::kBytes));
   CUtensorMap q, k, v;
   BFB_TRY(make_map(&q, a.q, dtype, a.total_q, a.heads, a.dim, a.q_row, a.q_head));
   // without keys nothing is loaded, but the maps need an address
@@ -355,8 +358,6 @@ int launch(const Args& a, int dtype, cudaStream_t stream) {
   BFB_TRY(make_map(&v, a.total_k ? a.v : a.q, dtype, a.total_k, a.kv_heads, a.dim, a.v_row, a.v_head));
   const int64_t blocks = tile_bound(a.total_q, a.seqs, 2 * kTile) * a.heads;
   if (blocks > 0x7fffffff) return BFB_ERR_TOO_LARGE;
-  BFB_CUDA(cudaFuncSetAttribute(forward_kernel<T, DP>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                Layout<DP>::kBytes));
   forward_kernel<T, DP><<<(unsigned)blocks, kThreads, Layout<DP>::kBytes, stream>>>(a, q, k, v);
   BFB_CHECK_LAUNCH();
   return BFB_OK;

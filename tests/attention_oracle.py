@@ -11,6 +11,9 @@ dtype's largest absolute error where it underflows:
 * lse, delta and the scores are fp32; their error (a few 2^-24 times scores
   below 2^6 here, and exp2's 2^-22) is covered by 2^-14 relative to the sum of
   absolute terms.
+* Exponentials below fp32's smallest normal, 2^-126, are flushed to 0 (ex2 with
+  ftz): P's absolute error is at least that, whatever the dtype, and reaches dS
+  times |dP| + |delta|.
 * dS is rounded before dS K and dS^T Q; delta is made of the rounded o, so it
   carries the error of o times |dO|.
 """
@@ -20,6 +23,7 @@ import numpy as np
 import torch
 
 FP32 = 2.0 ** -14
+FLUSH = 2.0 ** -126
 
 
 def half_step(dtype):
@@ -27,7 +31,7 @@ def half_step(dtype):
 
 
 def underflow(dtype):
-    return torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2
+    return max(torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2, FLUSH)
 
 
 def attention(q, k, v, lens_q, lens_k, causal, scale, room_k=None, dout=None, dlse=None):
@@ -72,7 +76,7 @@ def attention(q, k, v, lens_q, lens_k, causal, scale, room_k=None, dout=None, dl
             ds = p * (dp - delta[:, None]) * scale
             d_tol = (g.abs() * o_tol).sum(1)
             ds_tol = (u * ds.abs() + p * d_tol[:, None] * abs(scale) + t +
-                      FP32 * p * (g.abs() @ z.abs().t() + delta.abs()[:, None]) * abs(scale))
+                      (FP32 * p + FLUSH) * (g.abs() @ z.abs().t() + delta.abs()[:, None]) * abs(scale))
             value['dq'][rows, h], tol['dq'][rows, h] = ds @ y, ds_tol @ y.abs()
             value['dk'][keys, m] += ds.t() @ x
             tol['dk'][keys, m] += ds_tol.t() @ x.abs()

@@ -28,7 +28,7 @@ NVCC = os.path.join(CUDA_HOME, 'bin', 'nvcc')
 GENCODE = ['-gencode', 'arch=compute_100a,code=sm_100a']
 CU_SOURCES = ['capi.cu', 'scan.cu', 'radix.cu', 'bev_pool.cu', 'voxelize.cu', 'scatter.cu', 'spconv.cu',
               'spconv_conv.cu', 'token_ops.cu', 'attention.cu',
-              'attention_fwd.cu', 'attention_bwd.cu']
+              'attention_fwd.cu', 'attention_bwd.cu', 'attention_rows.cu']
 
 
 def _headers() -> list[Path]:

@@ -37,6 +37,12 @@ int check_args(const Attn& a, int dtype) {
   return BFB_OK;
 }
 
+// Whether the queries are few enough for the kernel that is split over the
+// keys: up to two of its 16-row tiles for the average sequence and key head.
+bool few_rows(int64_t total_q, int64_t heads, int64_t kv_heads, int64_t seqs) {
+  return total_q * (heads / kv_heads) <= 32 * seqs;
+}
+
 Attn make(const void* q, const void* k, const void* v, const int64_t* strides, int64_t total_q, int64_t total_k,
           int64_t heads, int64_t kv_heads, int64_t dim, int64_t seqs, const int32_t* cu_q, const int32_t* cu_k,
           const int32_t* kv_lengths, int causal, double scale) {
@@ -67,6 +73,8 @@ extern "C" int bfb_packed_attention_workspace_size(int64_t total_q, int64_t tota
   if (backward) {
     c.take<float>((size_t)(total_q * heads));
     c.take<float>((size_t)(total_q * heads));
+  } else if (few_rows(total_q, heads, kv_heads, seqs)) {
+    c.take<float>(attn::rows_record_floats((int)dim));
   }
   *bytes = c.bytes();
   return BFB_OK;
@@ -85,6 +93,13 @@ extern "C" int bfb_packed_attention(const void* q_dev, const void* k_dev, const 
   a.lse = lse_dev;
   BFB_TRY(check_args(a, dtype));
   if (total_q == 0) return BFB_OK;
+  if (few_rows(total_q, heads, kv_heads, seqs)) {
+    size_t need = 0;
+    BFB_TRY(bfb_packed_attention_workspace_size(total_q, total_k, heads, kv_heads, dim, seqs, 0, &need));
+    if (!workspace_dev || workspace_bytes < need) return BFB_ERR_WORKSPACE;
+    Carver c(workspace_dev);
+    return attn::forward_rows(a, dtype, c.take<float>(attn::rows_record_floats(a.dim)), as_stream(stream));
+  }
   return attn::forward_sm100(a, dtype, as_stream(stream));
 }
 

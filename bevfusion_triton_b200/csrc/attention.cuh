@@ -103,6 +103,10 @@ int make_map(CUtensorMap* map, const void* base, int dtype, int64_t rows, int he
 
 int forward_sm100(const Args& a, int dtype, cudaStream_t stream);
 int backward_sm100(const Args& a, int dtype, cudaStream_t stream);
+// Few queries against long keys, split over the keys; `records`: its workspace.
+constexpr int kRowsBlocks = 148 * 2;  // two blocks fit an SM
+size_t rows_record_floats(int dim);
+int forward_rows(const Args& a, int dtype, float* records, cudaStream_t stream);
 int timeouts_forward(uint64_t* count, int reset);
 int timeouts_backward(uint64_t* count, int reset);
 

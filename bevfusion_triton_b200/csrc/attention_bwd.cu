@@ -12,6 +12,12 @@
 // worked by two warpgroups, one per 64 columns, with 64 values per thread.
 // dS carries the scale before it is rounded: in fp16 it then overflows only
 // where the gradient itself is near to.
+//
+// delta comes from the rounded o, an error of 2^-9 (bf16) of |dO| |o| that all
+// of a row's dS share.  Over many keys it is lost among them; over few keys,
+// where P is near 1 and dS near 0, it would be most of the result.  So where a
+// sequence's keys fit one tile the dQ kernel sums delta = rowsum(P dP) - dlse
+// in fp32 itself, and leaves it for the dK and dV kernel, which runs second.
 #include <algorithm>
 
 #include "attention.cuh"
@@ -47,7 +53,7 @@ struct Shared {
   uint32_t tmem;
   int part, tile, lq, lk, room;
   int64_t q0, k0;
-  float lse2[kFirst][kTile], delta[kSecond][kTile];
+  float lse2[kFirst][kTile], delta[kSecond][kTile];  // dQ: delta's first half row from each warpgroup
 };
 
 template <int DP>
@@ -432,7 +438,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, mine = lanes + wg * kHalf;
     const float c = a.scale * kLog2e;
     const int64_t at = (int64_t)h * a.total_q + s.q0 + i;
-    const float lse2 = i < lq ? a.lse2[at] : INFINITY, delta = i < lq ? a.delta[at] : 0.f;
+    const float lse2 = i < lq ? a.lse2[at] : INFINITY;
+    const bool exact = lk <= kTile;  // one tile of keys: delta is summed here
+    float delta = i < lq && !exact ? a.delta[at] : 0.f;
     const int sees = seen(i), warp_sees = seen(i - lane);
     bool ok = true;
     for (int j = 0; j < n; ++j) {
@@ -456,6 +464,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       tmem_ld32(tdp + mine + 32, x + 32);
       tmem_ld_wait32(x);
       tmem_ld_wait32(x + 32);
+      if (exact) {
+        float part = 0.f;
+#pragma unroll
+        for (int e = 0; e < kHalf; ++e) part += e < limit ? p[e] * __uint_as_float(x[e]) : 0.f;
+        s.delta[wg][row] = part;
+        asm volatile("bar.sync 1, 256;" ::: "memory");  // the two warpgroups
+        if (i < lq) {
+          delta = a.scale * (s.delta[0][row] + s.delta[1][row] - (a.dlse ? a.dlse[at] : 0.f));
+          if (wg == 0) a.delta[at] = delta;
+        }
+      }
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
         uint32_t w[16];
@@ -591,12 +610,12 @@ int launch(const Args& a, int dtype, cudaStream_t stream) {
     rows_kernel<T><<<(unsigned)row_blocks, 256, 0, stream>>>(a, lanes);
     BFB_CHECK_LAUNCH();
   }
-  if (a.total_k > 0) {
-    dkv_kernel<T, DP><<<(unsigned)k_blocks, kThreads, kBytes, stream>>>(a, q, k, v, g);
-    BFB_CHECK_LAUNCH();
-  }
   if (a.total_q > 0) {
     dq_kernel<T, DP><<<(unsigned)q_blocks, kThreads, kBytes, stream>>>(a, q, k, v, g);
+    BFB_CHECK_LAUNCH();
+  }
+  if (a.total_k > 0) {
+    dkv_kernel<T, DP><<<(unsigned)k_blocks, kThreads, kBytes, stream>>>(a, q, k, v, g);
     BFB_CHECK_LAUNCH();
   }
   return BFB_OK;

@@ -6,6 +6,7 @@
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
 #include <map>
@@ -1115,4 +1116,225 @@ TORCH_LIBRARY_IMPL(bfb_b200, CUDA, m) {
   m.impl("qk_norm_rotary", &qk_norm_rotary);
   m.impl("qk_norm_rotary_backward", &qk_norm_rotary_backward);
   m.impl("residual_dropout", &residual_dropout);
+}
+
+// Autograd of the attention-block operators, in C++ so that a small training
+// step is not spent in the interpreter (a forward and backward of the three
+// through torch.library.register_autograd cost over 100 us each on the host).
+// The formulas call the ops through the dispatcher, so tracing sees them.
+namespace {
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+bool wants_grad(std::initializer_list<const at::Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const at::Tensor* t : ts)
+    if (t->defined() && t->requires_grad()) return true;
+  return false;
+}
+
+const at::Tensor& or_none(const c10::optional<at::Tensor>& t) {
+  static const at::Tensor none;
+  return t.has_value() ? *t : none;
+}
+c10::optional<at::Tensor> or_null(const at::Tensor& t) {
+  return t.defined() ? c10::optional<at::Tensor>(t) : c10::nullopt;
+}
+
+template <class F>
+auto op_handle(const char* name) {
+  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
+}
+
+std::tuple<at::Tensor, at::Tensor> call_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                                  const at::Tensor& cu_q, const at::Tensor& cu_k,
+                                                  const c10::optional<at::Tensor>& lengths, bool causal,
+                                                  double scale) {
+  static const auto op = op_handle<decltype(packed_attention)>("bfb_b200::packed_attention");
+  at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(q, k, v, cu_q, cu_k, lengths, causal, scale);
+}
+
+[[noreturn]] void no_second(const char* name) {
+  TORCH_CHECK_NOT_IMPLEMENTED(false, name, " has no second derivative");
+  std::abort();  // not reached: the check throws
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> call_attention_backward(
+    const at::Tensor& dout, const c10::optional<at::Tensor>& dlse, const at::Tensor& q, const at::Tensor& k,
+    const at::Tensor& v, const at::Tensor& out, const at::Tensor& lse, const at::Tensor& cu_q, const at::Tensor& cu_k,
+    const c10::optional<at::Tensor>& lengths, bool causal, double scale) {
+  static const auto op = op_handle<decltype(packed_attention_backward)>("bfb_b200::packed_attention_backward");
+  at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(dout, dlse, q, k, v, out, lse, cu_q, cu_k, lengths, causal, scale);
+}
+
+// Under create_graph the gradients say that they cannot be differentiated again.
+struct AttentionSecond : torch::autograd::Function<AttentionSecond> {
+  static variable_list forward(AutogradContext*, const at::Tensor& dout, const c10::optional<at::Tensor>& dlse,
+                               const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& out,
+                               const at::Tensor& lse, const at::Tensor& cu_q, const at::Tensor& cu_k,
+                               const c10::optional<at::Tensor>& lengths, bool causal, double scale) {
+    auto [dq, dk, dv] = call_attention_backward(dout, dlse, q, k, v, out, lse, cu_q, cu_k, lengths, causal, scale);
+    return {dq, dk, dv};
+  }
+  static variable_list backward(AutogradContext*, variable_list) { no_second("packed_attention"); }
+};
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor> attention_backward_autograd(
+    const at::Tensor& dout, const c10::optional<at::Tensor>& dlse, const at::Tensor& q, const at::Tensor& k,
+    const at::Tensor& v, const at::Tensor& out, const at::Tensor& lse, const at::Tensor& cu_q, const at::Tensor& cu_k,
+    const c10::optional<at::Tensor>& lengths, bool causal, double scale) {
+  if (!wants_grad({&dout, &or_none(dlse), &q, &k, &v, &out, &lse}))
+    return call_attention_backward(dout, dlse, q, k, v, out, lse, cu_q, cu_k, lengths, causal, scale);
+  auto r = AttentionSecond::apply(dout, dlse, q, k, v, out, lse, cu_q, cu_k, lengths, causal, scale);
+  return {r[0], r[1], r[2]};
+}
+
+struct AttentionGrad : torch::autograd::Function<AttentionGrad> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                               const at::Tensor& cu_q, const at::Tensor& cu_k,
+                               const c10::optional<at::Tensor>& lengths, bool causal, double scale) {
+    auto [out, lse] = call_attention(q, k, v, cu_q, cu_k, lengths, causal, scale);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({q, k, v, out, lse, cu_q, cu_k, or_none(lengths)});
+    ctx->saved_data["causal"] = causal;
+    ctx->saved_data["scale"] = scale;
+    return {out, lse};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    static const auto op = op_handle<decltype(packed_attention_backward)>("bfb_b200::packed_attention_backward");
+    const auto s = ctx->get_saved_variables();
+    const auto dout = grads[0].defined() ? grads[0] : at::zeros_like(s[3]);
+    auto [dq, dk, dv] = op.call(dout, or_null(grads[1]), s[0], s[1], s[2], s[3], s[4], s[5], s[6], or_null(s[7]),
+                                ctx->saved_data["causal"].toBool(), ctx->saved_data["scale"].toDouble());
+    return {dq, dk, dv, {}, {}, {}, {}, {}};
+  }
+};
+
+std::tuple<at::Tensor, at::Tensor> attention_autograd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                                      const at::Tensor& cu_q, const at::Tensor& cu_k,
+                                                      const c10::optional<at::Tensor>& lengths, bool causal,
+                                                      double scale) {
+  if (!wants_grad({&q, &k, &v})) return call_attention(q, k, v, cu_q, cu_k, lengths, causal, scale);
+  auto r = AttentionGrad::apply(q, k, v, cu_q, cu_k, lengths, causal, scale);
+  return {r[0], r[1]};
+}
+
+std::tuple<at::Tensor, at::Tensor> call_rotary(const at::Tensor& q, const at::Tensor& k, const at::Tensor& positions,
+                                               const at::Tensor& inv_freq, at::IntArrayRef sections,
+                                               const c10::optional<at::Tensor>& qw,
+                                               const c10::optional<at::Tensor>& kw, double eps, bool interleaved) {
+  static const auto op = op_handle<decltype(qk_norm_rotary)>("bfb_b200::qk_norm_rotary");
+  at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(q, k, positions, inv_freq, sections, qw, kw, eps, interleaved);
+}
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> call_rotary_backward(
+    const at::Tensor& gq, const at::Tensor& gk, const at::Tensor& q, const at::Tensor& k, const at::Tensor& positions,
+    const at::Tensor& inv_freq, at::IntArrayRef sections, const c10::optional<at::Tensor>& qw,
+    const c10::optional<at::Tensor>& kw, double eps, bool interleaved) {
+  static const auto op = op_handle<decltype(qk_norm_rotary_backward)>("bfb_b200::qk_norm_rotary_backward");
+  at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(gq, gk, q, k, positions, inv_freq, sections, qw, kw, eps, interleaved);
+}
+
+struct RotarySecond : torch::autograd::Function<RotarySecond> {
+  static variable_list forward(AutogradContext*, const at::Tensor& gq, const at::Tensor& gk, const at::Tensor& q,
+                               const at::Tensor& k, const at::Tensor& positions, const at::Tensor& inv_freq,
+                               at::IntArrayRef sections, const c10::optional<at::Tensor>& qw,
+                               const c10::optional<at::Tensor>& kw, double eps, bool interleaved) {
+    auto [dq, dk, dqw, dkw] = call_rotary_backward(gq, gk, q, k, positions, inv_freq, sections, qw, kw, eps,
+                                                   interleaved);
+    return {dq, dk, dqw, dkw};
+  }
+  static variable_list backward(AutogradContext*, variable_list) { no_second("qk_norm_rotary"); }
+};
+
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> rotary_backward_autograd(
+    const at::Tensor& gq, const at::Tensor& gk, const at::Tensor& q, const at::Tensor& k, const at::Tensor& positions,
+    const at::Tensor& inv_freq, at::IntArrayRef sections, const c10::optional<at::Tensor>& qw,
+    const c10::optional<at::Tensor>& kw, double eps, bool interleaved) {
+  if (!wants_grad({&gq, &gk, &q, &k, &or_none(qw), &or_none(kw)}))
+    return call_rotary_backward(gq, gk, q, k, positions, inv_freq, sections, qw, kw, eps, interleaved);
+  auto r = RotarySecond::apply(gq, gk, q, k, positions, inv_freq, sections, qw, kw, eps, interleaved);
+  return {r[0], r[1], r[2], r[3]};
+}
+
+struct RotaryGrad : torch::autograd::Function<RotaryGrad> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k,
+                               const at::Tensor& positions, const at::Tensor& inv_freq, at::IntArrayRef sections,
+                               const c10::optional<at::Tensor>& qw, const c10::optional<at::Tensor>& kw, double eps,
+                               bool interleaved) {
+    auto [qo, ko] = call_rotary(q, k, positions, inv_freq, sections, qw, kw, eps, interleaved);
+    ctx->save_for_backward({q, k, positions, inv_freq, or_none(qw), or_none(kw)});
+    ctx->saved_data["sections"] = sections.vec();
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["interleaved"] = interleaved;
+    return {qo, ko};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    static const auto op = op_handle<decltype(qk_norm_rotary_backward)>("bfb_b200::qk_norm_rotary_backward");
+    const auto s = ctx->get_saved_variables();
+    const auto sections = ctx->saved_data["sections"].toIntVector();
+    auto [dq, dk, dqw, dkw] =
+        op.call(grads[0], grads[1], s[0], s[1], s[2], s[3], sections, or_null(s[4]), or_null(s[5]),
+                ctx->saved_data["eps"].toDouble(), ctx->saved_data["interleaved"].toBool());
+    return {dq, dk, {}, {}, {}, s[4].defined() ? dqw : at::Tensor(), s[5].defined() ? dkw : at::Tensor(), {}, {}};
+  }
+};
+
+std::tuple<at::Tensor, at::Tensor> rotary_autograd(const at::Tensor& q, const at::Tensor& k,
+                                                   const at::Tensor& positions, const at::Tensor& inv_freq,
+                                                   at::IntArrayRef sections, const c10::optional<at::Tensor>& qw,
+                                                   const c10::optional<at::Tensor>& kw, double eps,
+                                                   bool interleaved) {
+  if (!wants_grad({&q, &k, &or_none(qw), &or_none(kw)}))
+    return call_rotary(q, k, positions, inv_freq, sections, qw, kw, eps, interleaved);
+  auto r = RotaryGrad::apply(q, k, positions, inv_freq, sections, qw, kw, eps, interleaved);
+  return {r[0], r[1]};
+}
+
+at::Tensor call_dropout(const at::Tensor& x, const c10::optional<at::Tensor>& residual, double p,
+                        const at::Tensor& seed) {
+  static const auto op = op_handle<decltype(residual_dropout)>("bfb_b200::residual_dropout");
+  at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(x, residual, p, seed);
+}
+
+struct DropoutGrad : torch::autograd::Function<DropoutGrad> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const c10::optional<at::Tensor>& residual,
+                            double p, const at::Tensor& seed) {
+    ctx->save_for_backward({seed});
+    ctx->saved_data["p"] = p;
+    ctx->saved_data["residual"] = residual.has_value() && residual->defined();
+    return call_dropout(x, residual, p, seed);
+  }
+  // the same mask, drawn again; differentiable in its turn
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto s = ctx->get_saved_variables();
+    at::Tensor dx;
+    if (ctx->needs_input_grad(0)) {
+      static const auto op = op_handle<decltype(residual_dropout)>("bfb_b200::residual_dropout");
+      dx = op.call(grads[0], c10::nullopt, ctx->saved_data["p"].toDouble(), s[0]);
+    }
+    return {dx, ctx->saved_data["residual"].toBool() ? grads[0] : at::Tensor(), {}, {}};
+  }
+};
+
+at::Tensor dropout_autograd(const at::Tensor& x, const c10::optional<at::Tensor>& residual, double p,
+                            const at::Tensor& seed) {
+  if (!wants_grad({&x, &or_none(residual)})) return call_dropout(x, residual, p, seed);
+  return DropoutGrad::apply(x, residual, p, seed);
+}
+
+}  // namespace
+
+TORCH_LIBRARY_IMPL(bfb_b200, Autograd, m) {
+  m.impl("packed_attention", &attention_autograd);
+  m.impl("packed_attention_backward", &attention_backward_autograd);
+  m.impl("qk_norm_rotary", &rotary_autograd);
+  m.impl("qk_norm_rotary_backward", &rotary_backward_autograd);
+  m.impl("residual_dropout", &dropout_autograd);
 }

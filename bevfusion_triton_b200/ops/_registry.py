@@ -15,8 +15,9 @@ and registers the backward of the differentiable ones
   (ops/voxel/scatter_points.py:8-50, scatter_points_triton.py:348-424);
 * ``indice_conv`` -> ``indice_conv_backward`` and ``indice_maxpool`` ->
   ``indice_maxpool_backward`` (ops/spconv/functional.py:21-110);
-* ``packed_attention`` -> ``packed_attention_backward``, ``qk_norm_rotary`` ->
-  ``qk_norm_rotary_backward``, ``residual_dropout`` -> itself on the gradient.
+
+``packed_attention``, ``qk_norm_rotary`` and ``residual_dropout`` have theirs in
+``csrc/torch_ops.cpp``.
 
 Workspace sizes in the fake kernels come from the library's host-only size
 queries, so a traced plan tensor has exactly the size the real op returns.
@@ -280,51 +281,6 @@ def _register_autograd() -> None:
         return O.indice_maxpool_backward(features, out, grad.contiguous(), pairs, num), None, None, None
 
     torch.library.register_autograd('bfb_b200::indice_maxpool', pool_backward, setup_context=pool_setup)
-
-    # packed attention: gradients of q, k and v from those of out and lse
-    def attention_setup(ctx, inputs, output):
-        q, k, v, cu_q, cu_k, lengths, causal, scale = inputs
-        ctx.set_materialize_grads(False)
-        ctx.save_for_backward(q, k, v, *output, cu_q, cu_k, lengths)
-        ctx.how = (causal, scale)
-
-    def attention_backward(ctx, out_grad, lse_grad):
-        q, k, v, out, lse, cu_q, cu_k, lengths = ctx.saved_tensors
-        if out_grad is None:
-            out_grad = torch.zeros_like(out)
-        grads = O.packed_attention_backward(out_grad, lse_grad, q, k, v, out, lse, cu_q, cu_k, lengths, *ctx.how)
-        return (*grads, None, None, None, None, None)
-
-    torch.library.register_autograd('bfb_b200::packed_attention', attention_backward, setup_context=attention_setup)
-
-    # norm and rotary positions of queries and keys
-    def rotary_setup(ctx, inputs, output):
-        q, k, positions, inv_freq, sections, qw, kw, eps, interleaved = inputs
-        ctx.save_for_backward(q, k, positions, inv_freq, qw, kw)
-        ctx.how = (sections, eps, interleaved)
-
-    def rotary_backward(ctx, q_grad, k_grad):
-        q, k, positions, inv_freq, qw, kw = ctx.saved_tensors
-        sections, eps, interleaved = ctx.how
-        dq, dk, dqw, dkw = O.qk_norm_rotary_backward(q_grad, k_grad, q, k, positions, inv_freq, sections, qw, kw, eps,
-                                                     interleaved)
-        return dq, dk, None, None, None, None if qw is None else dqw, None if kw is None else dkw, None, None
-
-    torch.library.register_autograd('bfb_b200::qk_norm_rotary', rotary_backward, setup_context=rotary_setup)
-
-    # dropout onto a residual: the gradient goes through the same mask, drawn again
-    def dropout_setup(ctx, inputs, output):
-        _, residual, p, seed = inputs
-        ctx.save_for_backward(seed)
-        ctx.how = (p, residual is not None)
-
-    def dropout_backward(ctx, grad):
-        (seed,) = ctx.saved_tensors
-        p, has_residual = ctx.how
-        gx = O.residual_dropout(grad, None, p, seed) if ctx.needs_input_grad[0] else None
-        return gx, grad if has_residual else None, None, None
-
-    torch.library.register_autograd('bfb_b200::residual_dropout', dropout_backward, setup_context=dropout_setup)
 
 
 def register() -> None:

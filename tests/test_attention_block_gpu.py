@@ -339,6 +339,65 @@ def test_float_gradients_are_optional(cuda):
     assert not packed_attention(q, k, v, offsets([150])).requires_grad
 
 
+def test_single_key_has_no_gradient_through_its_score(cuda):
+    """One key: P = 1 whatever the score, so q and k get (to fp32's rounding) nothing, although o is rounded."""
+    lens = [1] * 50
+    q, k, v, g, _ = make(BF16, 2, 2, 128, lens, lens, seed=14)
+    x, y, z = (t.requires_grad_(True) for t in (q, k, v))
+    out = packed_attention(x, y, z, offsets(lens), causal=True)
+    dq, dk, dv = torch.autograd.grad(out, (x, y, z), g)
+    # |dP - delta| is below a few fp32 steps of sum |g| |v| < 2^9
+    assert float(dq.abs().max()) < 2.0 ** -10 and float(dk.abs().max()) < 2.0 ** -10
+    assert torch.equal(dv, g) and torch.equal(out.detach(), v.detach())
+
+
+@pytest.mark.parametrize('seqs', [31, 64, 100])
+@pytest.mark.parametrize('heads,kv', [(4, 4), (24, 2)])
+def test_many_streams(cuda, seqs, heads, kv):
+    """One to three queries for each of many sequences: cuts through groups, groups of two row tiles, empty caches."""
+    rng = np.random.default_rng(seqs)
+    lens_k = [int(n) for n in rng.integers(0, 700, seqs)]
+    lens_q = [int(n) for n in rng.integers(0, 3, seqs)]
+    both(BF16, heads, kv, 64, lens_q, lens_k, causal=True, spare=3, seed=seqs)
+    both(F16, heads, kv, 128, [1] * seqs, lens_k, causal=False, seed=seqs + 1)
+
+
+def test_second_derivative_is_refused(cuda):
+    q, k, v, g, _ = make(F16, 2, 2, 64, [20], [20])
+    q.requires_grad_(True)
+    (dq,) = torch.autograd.grad(packed_attention(q, k, v, offsets([20])), q, g, create_graph=True)
+    with pytest.raises(NotImplementedError):
+        dq.sum().backward()
+    x = torch.randn(4, 2, 16, device='cuda', requires_grad=True)
+    pos, freq = torch.zeros(4, 1, device='cuda'), torch.ones(8, device='cuda')
+    out, _ = qk_norm_rotary(x, x, pos, freq, (8,))
+    (dx,) = torch.autograd.grad(out.sum(), x, create_graph=True)
+    with pytest.raises(NotImplementedError):
+        dx.sum().backward()
+    y = residual_dropout(x, x, 0.5, torch.zeros(2, dtype=torch.int64, device='cuda'))
+    (dx,) = torch.autograd.grad(y, x, torch.ones_like(y).requires_grad_(True), create_graph=True)
+    assert dx.requires_grad  # linear in the gradient: differentiable again
+
+
+def test_compiled(cuda):
+    """torch.compile traces through the three operators, forward and backward."""
+    q, k, v, g, _ = make(F16, 4, 2, 64, [40, 25], [40, 25], seed=15)
+    cu, seed = offsets([40, 25]), torch.tensor([3, 4], device='cuda')
+    pos, freq = torch.arange(65, device='cuda')[:, None], torch.rand(32, device='cuda')
+    w = torch.ones(64, device='cuda', requires_grad=True)
+
+    def block(q, k, v, w):
+        a, b = qk_norm_rotary(q, k, pos, freq, (32,), w, w)
+        return residual_dropout(packed_attention(a, b, v, cu, causal=True), q, 0.2, seed)
+
+    leaves = [t.requires_grad_(True) for t in (q, k, v)] + [w]
+    want = block(*leaves)
+    got = torch.compile(block, backend='aot_eager', fullgraph=True)(*leaves)
+    assert torch.equal(got, want)
+    for a, b in zip(torch.autograd.grad(got, leaves, g), torch.autograd.grad(want, leaves, g)):
+        assert torch.equal(a, b)
+
+
 # ----------------------------------------------------------- norm and rotary
 def rotary_case(dtype, tokens, heads, kv, dim, sections, norm, positions, interleaved, reach, seed=0, eps=1e-6):
     g = torch.Generator(device='cuda').manual_seed(seed)

@@ -82,21 +82,39 @@ __device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* map, 
 
 // dst += A B over 128 rows of B (A in tensor memory, B's rows along K).
 template <int DP, bool kBf16>
-__device__ __forceinline__ void product_rows(uint32_t dst, uint32_t a, uint32_t b, bool first) {
+__device__ __forceinline__ void product_rows(bool leader, uint32_t dst, uint32_t a, uint32_t b, bool first) {
+  const TileDesc bd(b, Layout<DP>::kPanel);
+  if (leader) {
 #pragma unroll
-  for (int c = 0; c < kTile / 16; ++c)
-    mma_ts(dst, a + half_step(c), tile_desc(b + c * 2048, Layout<DP>::kPanel), mma_desc(kBf16, DP, true),
-           !first || c > 0);
+    for (int c = 0; c < kTile / 16; ++c)
+      mma_ts(dst, a + half_step(c), bd.at(c * 2048), mma_desc(kBf16, DP, true), !first || c > 0);
+  }
 }
 // dst = A B^T over the columns of two tiles.
 template <int DP, bool kBf16>
-__device__ __forceinline__ void product_cols(uint32_t dst, uint32_t a, uint32_t b) {
+__device__ __forceinline__ void product_cols(bool leader, uint32_t dst, uint32_t a, uint32_t b) {
+  const TileDesc ad(a, 16), bd(b, 16);
+  if (leader) {
 #pragma unroll
-  for (int c = 0; c < DP / 16; ++c) {
-    const uint32_t off = (c / 4) * Layout<DP>::kPanel + (c % 4) * 32;
-    mma_ss(dst, tile_desc(a + off, 16), tile_desc(b + off, 16), mma_desc(kBf16, kTile, false), c > 0);
+    for (int c = 0; c < DP / 16; ++c) {
+      const uint32_t off = (c / 4) * Layout<DP>::kPanel + (c % 4) * 32;
+      mma_ss(dst, ad.at(off), bd.at(off), mma_desc(kBf16, kTile, false), c > 0);
+    }
   }
 }
+
+// Position in a ring of N stages.
+template <int N>
+struct Ring {
+  int stage = 0;
+  uint32_t phase = 0;
+  __device__ __forceinline__ void step() {
+    if (++stage == N) {
+      stage = 0;
+      phase ^= 1;
+    }
+  }
+};
 
 // `cols` fp32 columns of a 128-row sum from tensor memory, as 16-bit values
 // [col0, col0 + cols) of a row of [rows, heads, dim].
@@ -163,8 +181,8 @@ __device__ __forceinline__ bool setup(Shared& s, const Args& a, int64_t item) {
       }
       bar_init(&s.s_full, 1);
       bar_init(&s.dp_full, 1);
-      bar_init(&s.p_ready, 2 * kTile);
-      bar_init(&s.ds_ready, 2 * kTile);
+      bar_init(&s.p_ready, 8);  // one arrival of each warp
+      bar_init(&s.ds_ready, 8);
       bar_init(&s.done, 1);
       bar_init(&s.tail, 1);
       fence_bar_init();
@@ -190,15 +208,23 @@ __device__ __forceinline__ void tmem_end(Shared& s, int warp) {
   }
 }
 
-// One warp's load of a ring's stage: waits for the stage, fetches `tile`'s
-// rows by TMA, has `extra` fill what goes with them, clears the rows from
-// `valid` on (kClear), and signals `full` (two arrivals).
-template <int DP, bool kClear, class F>
+// One warp's load of a ring's stage: waits for the stage, fetches the rows by
+// TMA with (src, not NULL) one value for each, negated, `past` from row
+// `valid` on, clears the rows from there on (kClear), and signals `full` (two
+// arrivals).  The values are fetched before the wait, all at once: one after
+// another behind it, their latencies were most of a step.
+template <int DP, bool kClear>
 __device__ __forceinline__ bool load_stage(uint8_t* dst, const CUtensorMap* map, int head, int64_t row, int valid,
                                            uint64_t* full, uint64_t* empty, uint32_t parity, uint64_t* tail,
-                                           uint32_t& tails, F extra) {
+                                           uint32_t& tails, const float* src = nullptr, float* values = nullptr,
+                                           float past = 0.f) {
   const int lane = threadIdx.x & 31;
   bool ok = true;
+  float x[4];
+  if (src) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = lane + 32 * e < valid ? -src[lane + 32 * e] : past;
+  }
   if (lane == 0) ok = bar_wait(empty, parity ^ 1, &g_timeouts);
   if (!__shfl_sync(0xffffffffu, ok, 0)) return false;
   const bool clear = kClear && valid < kTile;
@@ -207,7 +233,10 @@ __device__ __forceinline__ bool load_stage(uint8_t* dst, const CUtensorMap* map,
     bar_expect(bar, Layout<DP>::kTileBytes);
     load_tile<DP>(dst, map, head, row, bar);
   }
-  extra();
+  if (src) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) values[lane + 32 * e] = x[e];
+  }
   if (clear) {
     ok = bar_wait(tail, tails & 1, &g_timeouts);
     ++tails;
@@ -250,7 +279,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ __align__(1024) uint8_t tiles[];
   Shared& s = *reinterpret_cast<Shared*>(tiles + L::kTiles * L::kTileBytes);
   uint8_t *sk = tiles, *sv = sk + L::kTileBytes, *sq = sv + L::kTileBytes, *sg = sq + kFirst * L::kTileBytes;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const int m = blockIdx.x % a.kv_heads, group = a.heads / a.kv_heads;
   if (!setup<true>(s, a, blockIdx.x / a.kv_heads)) return;
   const uint32_t tmem = tmem_start(s, warp);
@@ -265,7 +294,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     regs_grow<208>();
     const int wg = warp >> 2, row = threadIdx.x & (kTile - 1), j = j0 + row;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, mine = lanes + wg * kHalf;
-    const float c = a.scale * kLog2e;
+    const float2 c2 = make_float2(a.scale * kLog2e, a.scale * kLog2e), scale2 = make_float2(a.scale, a.scale);
     bool ok = true;
     int tile = 0;
     for (int i = 0; i < n; ++i) {
@@ -281,15 +310,25 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (++tile == per_head) tile = 0;
       const int from = j - shift - q;
       const bool masked = a.causal && j0 + kTile - 1 - shift - q > 0;
-      const float* lse2 = s.lse2[sa] + wg * kHalf;
-      const float* delta = s.delta[sb] + wg * kHalf;
+      const float4* lse2 = reinterpret_cast<const float4*>(s.lse2[sa] + wg * kHalf);
+      const float4* delta = reinterpret_cast<const float4*>(s.delta[sb] + wg * kHalf);
       tmem_ld_wait32(x);
       tmem_ld_wait32(x + 32);
       float p[kHalf];
 #pragma unroll
-      for (int e = 0; e < kHalf; ++e) {
-        p[e] = exp2_approx(fmaf(__uint_as_float(x[e]), c, -lse2[e]));
-        if (masked && e < from) p[e] = 0.f;
+      for (int e = 0; e < kHalf; e += 4) {
+        const float4 l = lse2[e / 4];  // negative
+        const float2 u = fma2(pair_of(x + e), c2, make_float2(l.x, l.y));
+        const float2 v = fma2(pair_of(x + e + 2), c2, make_float2(l.z, l.w));
+        p[e] = exp2_approx(u.x);
+        p[e + 1] = exp2_approx(u.y);
+        p[e + 2] = exp2_approx(v.x);
+        p[e + 3] = exp2_approx(v.y);
+      }
+      if (masked) {
+#pragma unroll
+        for (int e = 0; e < kHalf; ++e)
+          if (e < from) p[e] = 0.f;
       }
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
@@ -300,7 +339,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       tmem_st_wait();
       tc_fence_before();
-      bar_arrive(&s.p_ready);
+      bar_arrive_warp(&s.p_ready);
       if (!(ok = bar_wait(&s.b_full[sb], (i / kSecond) & 1, &g_timeouts) && bar_wait(&s.dp_full, i & 1, &g_timeouts)))
         break;
       tc_fence_after();
@@ -312,21 +351,25 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int b = 0; b < 2; ++b) {
         uint32_t w[16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
+        for (int e = 0; e < 16; e += 2) {
           const int at = 32 * b + 2 * e;
-          float u = p[at] * fmaf(__uint_as_float(x[at]), a.scale, -delta[at]);
-          float v = p[at + 1] * fmaf(__uint_as_float(x[at + 1]), a.scale, -delta[at + 1]);
+          const float4 d = delta[at / 4];  // negative
+          float2 u = mul2(make_float2(p[at], p[at + 1]), fma2(pair_of(x + at), scale2, make_float2(d.x, d.y)));
+          float2 v = mul2(make_float2(p[at + 2], p[at + 3]), fma2(pair_of(x + at + 2), scale2, make_float2(d.z, d.w)));
           if (masked) {
-            if (at < from) u = 0.f;
-            if (at + 1 < from) v = 0.f;
+            if (at < from) u.x = 0.f;
+            if (at + 1 < from) u.y = 0.f;
+            if (at + 2 < from) v.x = 0.f;
+            if (at + 3 < from) v.y = 0.f;
           }
-          w[e] = pack2<T>(u, v);
+          w[e] = pack2<T>(u.x, u.y);
+          w[e + 1] = pack2<T>(v.x, v.y);
         }
         tmem_st16(tdp + mine + 16 * b, w);
       }
       tmem_st_wait();
       tc_fence_before();
-      bar_arrive(&s.ds_ready);
+      bar_arrive_warp(&s.ds_ready);
     }
     if (ok && (n == 0 || bar_wait(&s.done, 0, &g_timeouts))) {
       tc_fence_after();
@@ -335,43 +378,48 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     regs_shrink<88>();
-    if (warp == 8 && lane == 0 && n > 0) {
-      const uint32_t ka = smem_u32(sk), va = smem_u32(sv);
-      auto q_at = [&](int i) { return smem_u32(sq + (i % kFirst) * L::kTileBytes); };
-      auto g_at = [&](int i) { return smem_u32(sg + (i % kSecond) * L::kTileBytes); };
-      auto q_full = [&](int i) { return bar_wait(&s.a_full[i % kFirst], (i / kFirst) & 1, &g_timeouts); };
-      auto g_full = [&](int i) { return bar_wait(&s.b_full[i % kSecond], (i / kSecond) & 1, &g_timeouts); };
-      bool ok = bar_wait(&s.own_full, 0, &g_timeouts) && q_full(0) && g_full(0);
+    if (warp == 8 && n > 0) {
+      const bool leader = elect_one();
+      const uint32_t ka = smem_u32(sk), va = smem_u32(sv), q_addr = smem_u32(sq), g_addr = smem_u32(sg);
+      Ring<kFirst> qr;  // of the next scores
+      Ring<kSecond> gr;
+      bool ok = bar_wait(&s.own_full, 0, &g_timeouts) && bar_wait(&s.a_full[0], 0, &g_timeouts) &&
+                bar_wait(&s.b_full[0], 0, &g_timeouts);
       if (ok) {
         tc_fence_after();
-        product_cols<DP, kBf16>(ts, ka, q_at(0));
-        mma_commit(&s.s_full);
-        product_cols<DP, kBf16>(tdp, va, g_at(0));
-        mma_commit(&s.dp_full);
+        product_cols<DP, kBf16>(leader, ts, ka, q_addr);
+        if (leader) mma_commit(&s.s_full);
+        product_cols<DP, kBf16>(leader, tdp, va, g_addr);
+        if (leader) mma_commit(&s.dp_full);
       }
       for (int i = 0; i < n && ok; ++i) {
         const bool more = i + 1 < n;
+        const int qs = qr.stage, gs = gr.stage;
+        const uint32_t q_now = q_addr + qs * L::kTileBytes, g_now = g_addr + gs * L::kTileBytes;
+        qr.step();
+        gr.step();
         if (!(ok = bar_wait(&s.p_ready, i & 1, &g_timeouts))) break;
         tc_fence_after();
-        product_rows<DP, kBf16>(tdv, ts, g_at(i), i == 0);
+        product_rows<DP, kBf16>(leader, tdv, ts, g_now, i == 0);
         if (more) {
-          if (!(ok = q_full(i + 1))) break;
-          product_cols<DP, kBf16>(ts, ka, q_at(i + 1));
-          mma_commit(&s.s_full);
+          if (!(ok = bar_wait(&s.a_full[qr.stage], qr.phase, &g_timeouts))) break;
+          product_cols<DP, kBf16>(leader, ts, ka, q_addr + qr.stage * L::kTileBytes);
+          if (leader) mma_commit(&s.s_full);
         }
         if (!(ok = bar_wait(&s.ds_ready, i & 1, &g_timeouts))) break;
         tc_fence_after();
-        product_rows<DP, kBf16>(tdk, tdp, q_at(i), i == 0);
-        // both: the threads are done with lse2 and delta, too
-        mma_commit(&s.a_empty[i % kFirst]);
-        mma_commit(&s.b_empty[i % kSecond]);
+        product_rows<DP, kBf16>(leader, tdk, tdp, q_now, i == 0);
+        if (leader) {  // both: the threads are done with lse2 and delta, too
+          mma_commit(&s.a_empty[qs]);
+          mma_commit(&s.b_empty[gs]);
+        }
         if (more) {
-          if (!(ok = g_full(i + 1))) break;
-          product_cols<DP, kBf16>(tdp, va, g_at(i + 1));
-          mma_commit(&s.dp_full);
+          if (!(ok = bar_wait(&s.b_full[gr.stage], gr.phase, &g_timeouts))) break;
+          product_cols<DP, kBf16>(leader, tdp, va, g_addr + gr.stage * L::kTileBytes);
+          if (leader) mma_commit(&s.dp_full);
         }
       }
-      mma_commit(&s.done);
+      if (leader) mma_commit(&s.done);
       bar_wait(&s.done, 0, &g_timeouts);  // nothing leaves before its products are done
     } else if (warp == 9 && n > 0) {
       if (lane == 0) {
@@ -386,17 +434,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int64_t at = (int64_t)h * a.total_q + s.q0 + q;
         // rows past the sequence: P = exp2(-inf) = 0
         if (!load_stage<DP, true>(sq + sa * L::kTileBytes, &q_map, h, s.q0 + q, valid, &s.a_full[sa], &s.a_empty[sa],
-                                  (i / kFirst) & 1, &s.tail, tails, [&] {
-                                    for (int r = lane; r < kTile; r += 32)
-                                      s.lse2[sa][r] = r < valid ? a.lse2[at + r] : INFINITY;
-                                  }))
+                                  (i / kFirst) & 1, &s.tail, tails, a.lse2 + at, s.lse2[sa], -INFINITY))
           break;
         ++a_loads;
         if (!load_stage<DP, true>(sg + sb * L::kTileBytes, &g_map, h, s.q0 + q, valid, &s.b_full[sb], &s.b_empty[sb],
-                                  (i / kSecond) & 1, &s.tail, tails, [&] {
-                                    for (int r = lane; r < kTile; r += 32)
-                                      s.delta[sb][r] = r < valid ? a.delta[at + r] : 0.f;
-                                  }))
+                                  (i / kSecond) & 1, &s.tail, tails, a.delta + at, s.delta[sb], 0.f))
           break;
         if (++tile == per_head) {
           tile = 0;
@@ -423,7 +465,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   extern __shared__ __align__(1024) uint8_t tiles[];
   Shared& s = *reinterpret_cast<Shared*>(tiles + L::kTiles * L::kTileBytes);
   uint8_t *sq = tiles, *sg = sq + L::kTileBytes, *sk = sg + L::kTileBytes, *sv = sk + kFirst * L::kTileBytes;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const int h = blockIdx.x % a.heads, m = h / (a.heads / a.kv_heads);
   if (!setup<false>(s, a, blockIdx.x / a.heads)) return;
   const uint32_t tmem = tmem_start(s, warp);
@@ -436,7 +478,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     regs_grow<208>();
     const int wg = warp >> 2, row = threadIdx.x & (kTile - 1), i = i0 + row;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, mine = lanes + wg * kHalf;
-    const float c = a.scale * kLog2e;
+    const float2 c2 = make_float2(a.scale * kLog2e, a.scale * kLog2e), scale2 = make_float2(a.scale, a.scale);
     const int64_t at = (int64_t)h * a.total_q + s.q0 + i;
     const float lse2 = i < lq ? a.lse2[at] : INFINITY;
     const bool exact = lk <= kTile;  // one tile of keys: delta is summed here
@@ -452,12 +494,16 @@ __global__ void __launch_bounds__(kThreads, 1)
       tmem_ld_wait32(x);
       tmem_ld_wait32(x + 32);
       tc_fence_before();
-      bar_arrive(&s.p_ready);  // S is read
+      bar_arrive_warp(&s.p_ready);  // S is read
       const int limit = sees - j * kTile - wg * kHalf;
       const bool masked = warp_sees < j * kTile + wg * kHalf + kHalf;
       float p[kHalf];
 #pragma unroll
-      for (int e = 0; e < kHalf; ++e) p[e] = exp2_approx(fmaf(__uint_as_float(x[e]), c, -lse2));
+      for (int e = 0; e < kHalf; e += 2) {
+        const float2 u = fma2(pair_of(x + e), c2, make_float2(-lse2, -lse2));
+        p[e] = exp2_approx(u.x);
+        p[e + 1] = exp2_approx(u.y);
+      }
       if (!(ok = bar_wait(&s.dp_full, j & 1, &g_timeouts))) break;
       tc_fence_after();
       tmem_ld32(tdp + mine, x);
@@ -481,19 +527,19 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const int col = 32 * b + 2 * e;
-          float u = p[col] * fmaf(__uint_as_float(x[col]), a.scale, -delta);
-          float v = p[col + 1] * fmaf(__uint_as_float(x[col + 1]), a.scale, -delta);
+          float2 u = mul2(make_float2(p[col], p[col + 1]),
+                          fma2(pair_of(x + col), scale2, make_float2(-delta, -delta)));
           if (masked) {
-            if (col >= limit) u = 0.f;
-            if (col + 1 >= limit) v = 0.f;
+            if (col >= limit) u.x = 0.f;
+            if (col + 1 >= limit) u.y = 0.f;
           }
-          w[e] = pack2<T>(u, v);
+          w[e] = pack2<T>(u.x, u.y);
         }
         tmem_st16(tdp + mine + 16 * b, w);
       }
       tmem_st_wait();
       tc_fence_before();
-      bar_arrive(&s.ds_ready);
+      bar_arrive_warp(&s.ds_ready);
     }
     if (ok && (n == 0 || bar_wait(&s.done, 0, &g_timeouts))) {
       tc_fence_after();
@@ -502,42 +548,49 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     regs_shrink<88>();
-    if (warp == 8 && lane == 0 && n > 0) {
-      const uint32_t qa = smem_u32(sq), ga = smem_u32(sg);
-      auto k_at = [&](int j) { return smem_u32(sk + (j % kFirst) * L::kTileBytes); };
-      auto v_at = [&](int j) { return smem_u32(sv + (j % kSecond) * L::kTileBytes); };
-      auto k_full = [&](int j) { return bar_wait(&s.a_full[j % kFirst], (j / kFirst) & 1, &g_timeouts); };
-      auto v_full = [&](int j) { return bar_wait(&s.b_full[j % kSecond], (j / kSecond) & 1, &g_timeouts); };
-      bool ok = bar_wait(&s.own_full, 0, &g_timeouts) && k_full(0) && v_full(0);
+    if (warp == 8 && n > 0) {
+      const bool leader = elect_one();
+      const uint32_t qa = smem_u32(sq), ga = smem_u32(sg), k_addr = smem_u32(sk), v_addr = smem_u32(sv);
+      Ring<kFirst> kr;  // of the next scores
+      Ring<kSecond> vr;
+      bool ok = bar_wait(&s.own_full, 0, &g_timeouts) && bar_wait(&s.a_full[0], 0, &g_timeouts) &&
+                bar_wait(&s.b_full[0], 0, &g_timeouts);
       if (ok) {
         tc_fence_after();
-        product_cols<DP, kBf16>(ts, qa, k_at(0));
-        mma_commit(&s.s_full);
-        product_cols<DP, kBf16>(tdp, ga, v_at(0));
-        mma_commit(&s.dp_full);
-        mma_commit(&s.b_empty[0]);
+        product_cols<DP, kBf16>(leader, ts, qa, k_addr);
+        if (leader) mma_commit(&s.s_full);
+        product_cols<DP, kBf16>(leader, tdp, ga, v_addr);
+        if (leader) {
+          mma_commit(&s.dp_full);
+          mma_commit(&s.b_empty[0]);
+        }
       }
       for (int j = 0; j < n && ok; ++j) {
         const bool more = j + 1 < n;
+        const int ks = kr.stage;
+        kr.step();
+        vr.step();
         if (!(ok = bar_wait(&s.p_ready, j & 1, &g_timeouts))) break;
         tc_fence_after();
         if (more) {
-          if (!(ok = k_full(j + 1))) break;
-          product_cols<DP, kBf16>(ts, qa, k_at(j + 1));
-          mma_commit(&s.s_full);
+          if (!(ok = bar_wait(&s.a_full[kr.stage], kr.phase, &g_timeouts))) break;
+          product_cols<DP, kBf16>(leader, ts, qa, k_addr + kr.stage * L::kTileBytes);
+          if (leader) mma_commit(&s.s_full);
         }
         if (!(ok = bar_wait(&s.ds_ready, j & 1, &g_timeouts))) break;
         tc_fence_after();
-        product_rows<DP, kBf16>(tdq, tdp, k_at(j), j == 0);
-        mma_commit(&s.a_empty[j % kFirst]);
+        product_rows<DP, kBf16>(leader, tdq, tdp, k_addr + ks * L::kTileBytes, j == 0);
+        if (leader) mma_commit(&s.a_empty[ks]);
         if (more) {
-          if (!(ok = v_full(j + 1))) break;
-          product_cols<DP, kBf16>(tdp, ga, v_at(j + 1));
-          mma_commit(&s.dp_full);
-          mma_commit(&s.b_empty[(j + 1) % kSecond]);
+          if (!(ok = bar_wait(&s.b_full[vr.stage], vr.phase, &g_timeouts))) break;
+          product_cols<DP, kBf16>(leader, tdp, ga, v_addr + vr.stage * L::kTileBytes);
+          if (leader) {
+            mma_commit(&s.dp_full);
+            mma_commit(&s.b_empty[vr.stage]);
+          }
         }
       }
-      mma_commit(&s.done);
+      if (leader) mma_commit(&s.done);
       bar_wait(&s.done, 0, &g_timeouts);
     } else if (warp == 9 && n > 0) {
       if (lane == 0) {
@@ -551,11 +604,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int valid = lk - j * kTile, sa = j % kFirst, sb = j % kSecond;
         const int64_t k = s.k0 + (int64_t)j * kTile;
         if (!load_stage<DP, true>(sk + sa * L::kTileBytes, &k_map, m, k, valid, &s.a_full[sa], &s.a_empty[sa],
-                                  (j / kFirst) & 1, &s.tail, tails, [] {}))
+                                  (j / kFirst) & 1, &s.tail, tails))
           break;
         ++a_loads;
         if (!load_stage<DP, false>(sv + sb * L::kTileBytes, &v_map, m, k, valid, &s.b_full[sb], &s.b_empty[sb],
-                                   (j / kSecond) & 1, &s.tail, tails, [] {}))
+                                   (j / kSecond) & 1, &s.tail, tails))
           break;
       }
       if (lane == 0 && j < n) drain_loads(s, a_loads, j, tails);

@@ -57,7 +57,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* base = raw + (1024 - (smem_u32(raw) & 1023)) % 1024;
   uint8_t* sq = base;
   uint8_t* skv = base + 2 * L::kTileBytes;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
   const int h = blockIdx.x % a.heads, m = h / (a.heads / a.kv_heads);
 
   if (warp == 0) {
@@ -82,10 +82,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       for (int i = 0; i < 2; ++i) {
         bar_init(&s.s_full[i], 1);
-        bar_init(&s.p_ready[i], 2 * kTile);
-        bar_init(&s.grown[i], kTile);
+        bar_init(&s.p_ready[i], 8);  // a warp arrives once: 4 of softmax, 4 that scale O
+        bar_init(&s.grown[i], 4);
         bar_init(&s.o_full[i], 1);
-        bar_init(&s.sums[i], kTile);
+        bar_init(&s.sums[i], 4);
       }
       bar_init(&s.tail, 1);
       bar_init(&s.drained, 1);
@@ -153,34 +153,35 @@ __global__ void __launch_bounds__(kThreads, 1)
         top = now;
       }
       s.scale[t][row] = keep;
-      bar_arrive(&s.grown[t]);
+      bar_arrive_warp(&s.grown[t]);
       const float off = top == -INFINITY ? 0.f : -top;
-      float part[4] = {};
+      const float2 c2 = make_float2(c, c), off2 = make_float2(off, off);
+      float2 part[2] = {};
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
         uint32_t p[16];
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const int at = 32 * b + 2 * e;
-          float u = exp2_approx(fmaf(__uint_as_float(x[at]), c, off));
-          float v = exp2_approx(fmaf(__uint_as_float(x[at + 1]), c, off));
+          float2 u = fma2(pair_of(x + at), c2, off2);
+          u = make_float2(exp2_approx(u.x), exp2_approx(u.y));
           if (masked) {
-            if (at >= limit) u = 0.f;
-            if (at + 1 >= limit) v = 0.f;
+            if (at >= limit) u.x = 0.f;
+            if (at + 1 >= limit) u.y = 0.f;
           }
-          part[e & 1] += u;
-          part[2 + (e & 1)] += v;
-          p[e] = pack2<T>(u, v);
+          part[e & 1] = add2(part[e & 1], u);
+          p[e] = pack2<T>(u.x, u.y);
         }
         tmem_st16(ts + 16 * b, p);
       }
-      sum = sum * keep + ((part[0] + part[1]) + (part[2] + part[3]));
+      part[0] = add2(part[0], part[1]);
+      sum = sum * keep + (part[0].x + part[0].y);
       tmem_st_wait();
       tc_fence_before();
-      bar_arrive(&s.p_ready[t]);
+      bar_arrive_warp(&s.p_ready[t]);
     }
     s.sum[t][row] = sum;
-    bar_arrive(&s.sums[t]);
+    bar_arrive_warp(&s.sums[t]);
     if (i < lq)
       a.lse[(int64_t)h * a.total_q + s.q0 + i] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
   } else if (warp < 12) {
@@ -209,7 +210,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           tmem_st_wait();
           tc_fence_before();
         }
-        bar_arrive(&s.p_ready[t]);
+        bar_arrive_warp(&s.p_ready[t]);
       }
     }
     for (int t = 0; t < 2 && ok; ++t) {
@@ -246,49 +247,73 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     regs_shrink<48>();
-    if (warp == 12 && lane == 0 && n > 0) {
+    if (warp == 12 && n > 0) {
       // ---------------------------------------------------------- products
       constexpr uint32_t ds = mma_desc(kBf16, kTile, false), dv = mma_desc(kBf16, DP, true);
+      const bool leader = elect_one();
+      const uint32_t kv_addr = smem_u32(skv), q_addr = smem_u32(sq);
       auto score = [&](int t, int stage) {
-        const uint32_t qa = smem_u32(sq + t * L::kTileBytes), ka = smem_u32(skv + stage * L::kTileBytes);
+        const TileDesc qd(q_addr + t * L::kTileBytes, 16), kd(kv_addr + stage * L::kTileBytes, 16);
+        if (leader) {
 #pragma unroll
-        for (int c = 0; c < DP / 16; ++c) {
-          const uint32_t off = (c / 4) * L::kPanel + (c % 4) * 32;
-          mma_ss(tmem + t * kTile, tile_desc(qa + off, 16), tile_desc(ka + off, 16), ds, c > 0);
+          for (int c = 0; c < DP / 16; ++c) {
+            const uint32_t off = (c / 4) * L::kPanel + (c % 4) * 32;
+            mma_ss(tmem + t * kTile, qd.at(off), kd.at(off), ds, c > 0);
+          }
+          mma_commit(&s.s_full[t]);
         }
-        mma_commit(&s.s_full[t]);
       };
-      auto full = [&](int it) { return bar_wait(&s.kv_full[it % L::kStages], (it / L::kStages) & 1, &g_timeouts); };
-      bool ok = bar_wait(&s.q_full, 0, &g_timeouts) && full(0);
+      // the rings' next stage and phase
+      int stage = 0;
+      uint32_t phase = 0;
+      auto full = [&](int st, uint32_t ph) { return bar_wait(&s.kv_full[st], ph, &g_timeouts); };
+      auto step = [&] {
+        if (++stage == L::kStages) {
+          stage = 0;
+          phase ^= 1;
+        }
+      };
+      bool ok = bar_wait(&s.q_full, 0, &g_timeouts) && full(0, 0);
       if (ok) {
         tc_fence_after();
         if (n0 > 0) score(0, 0);
         if (n1 > 0) score(1, 0);
-        mma_commit(&s.kv_empty[0]);
+        if (leader) mma_commit(&s.kv_empty[0]);
       }
+      step();
       for (int j = 0; j < n && ok; ++j) {
-        const int vi = 2 * j + 1, ki = 2 * j + 2;
+        const int vs = stage;
+        if (!(ok = full(stage, phase))) break;
+        step();
+        const int ks = stage;
         const bool more = j + 1 < n;
-        if (!(ok = full(vi) && (!more || full(ki)))) break;
-        const uint32_t va = smem_u32(skv + (vi % L::kStages) * L::kTileBytes);
+        if (more) {
+          if (!(ok = full(stage, phase))) break;
+          step();
+        }
+        const TileDesc vd(kv_addr + vs * L::kTileBytes, L::kPanel);
+#pragma unroll
         for (int t = 0; t < 2; ++t) {
           const int steps = t ? n1 : n0;
           if (j >= steps) continue;
           if (!(ok = bar_wait(&s.p_ready[t], j & 1, &g_timeouts))) break;
           tc_fence_after();
+          if (leader) {
 #pragma unroll
-          for (int c = 0; c < kTile / 16; ++c)
-            mma_ts(tmem + 2 * kTile + t * DP, tmem + t * kTile + c * 8, tile_desc(va + c * 2048, L::kPanel), dv,
-                   j > 0 || c > 0);
-          if (j + 1 < steps) score(t, ki % L::kStages);
-          else mma_commit(&s.o_full[t]);
+            for (int c = 0; c < kTile / 16; ++c)
+              mma_ts(tmem + 2 * kTile + t * DP, tmem + t * kTile + c * 8, vd.at(c * 2048), dv, j > 0 || c > 0);
+          }
+          if (j + 1 < steps) score(t, ks);
+          else if (leader) mma_commit(&s.o_full[t]);
         }
         if (!ok) break;
-        mma_commit(&s.kv_empty[vi % L::kStages]);
-        if (more) mma_commit(&s.kv_empty[ki % L::kStages]);
+        if (leader) {
+          mma_commit(&s.kv_empty[vs]);
+          if (more) mma_commit(&s.kv_empty[ks]);
+        }
       }
       // nothing leaves before its products are done
-      mma_commit(&s.drained);
+      if (leader) mma_commit(&s.drained);
       bar_wait(&s.drained, 0, &g_timeouts);
     } else if (warp == 13 && n > 0) {
       // -------------------------------------------------------------- loads

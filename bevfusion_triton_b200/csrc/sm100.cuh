@@ -92,9 +92,24 @@ __device__ __forceinline__ void tmem_free(uint32_t tmem, uint32_t cols) {  // th
 // 64 columns one after another.  Read along its columns (K-major, 8-row groups
 // 1024 bytes apart) or along its rows (MN-major: `panel` bytes between groups
 // of 64 columns, 1024 between groups of 8 rows).
-__device__ __forceinline__ uint64_t tile_desc(uint32_t addr, uint32_t panel) {
-  return (uint64_t)((addr >> 4) & 0x3fff) | (uint64_t)((panel >> 4) & 0x3fff) << 16 | (uint64_t)(1024 >> 4) << 32 |
-         1ull << 46 /* version of sm_100 */ | 2ull << 61 /* 128-byte swizzle */;
+// Only the low word depends on the place, and steps within a tile add to it.
+struct TileDesc {
+  uint32_t lo;
+  __device__ __forceinline__ TileDesc(uint32_t addr, uint32_t panel) : lo((addr >> 4) | (panel >> 4) << 16) {}
+  __device__ __forceinline__ uint64_t at(uint32_t bytes) const {
+    constexpr uint64_t kHigh = (uint64_t)(1024 >> 4) << 32 | 1ull << 46 /* version of sm_100 */ |
+                               2ull << 61 /* 128-byte swizzle */;
+    return kHigh | (uint64_t)(lo + (bytes >> 4));
+  }
+};
+
+// True in one lane of a converged warp.  The warp that issues products runs
+// its loop with all lanes, so that addresses and descriptors stay in uniform
+// registers, and only the products themselves under this.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(one));
+  return one != 0;
 }
 
 // Instruction descriptor of kind::f16: fp32 accumulator, M = 128, B read
@@ -170,6 +185,42 @@ template <int N>
 __device__ __forceinline__ void regs_grow() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
 __device__ __forceinline__ void regs_shrink() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+// One arrival for a warp: 32 arrivals on one word would be taken one after
+// another.
+__device__ __forceinline__ void bar_arrive_warp(uint64_t* bar) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) bar_arrive(bar);
+}
+
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n .reg .b64 x, y, z, w;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n"
+      " fma.rn.f32x2 w, x, y, z;\n mov.b64 {%0, %1}, w;\n}\n"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n .reg .b64 x, y, w;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mul.rn.f32x2 w, x, y;\n"
+      " mov.b64 {%0, %1}, w;\n}\n"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n .reg .b64 x, y, w;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 w, x, y;\n"
+      " mov.b64 {%0, %1}, w;\n}\n"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 pair_of(const uint32_t* x) {
+  return make_float2(__uint_as_float(x[0]), __uint_as_float(x[1]));
+}
 
 __device__ __forceinline__ float exp2_approx(float x) {
   float y;

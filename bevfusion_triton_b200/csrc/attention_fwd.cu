@@ -15,6 +15,8 @@
 // Warps: 0-3 and 4-7 softmax of the two tiles, 8-11 scale O and write the
 // output, 12 issues the products, 13 loads by TMA.  While one tile is in its
 // softmax, the tensor core works on the other.
+#include <cfloat>
+
 #include "attention.cuh"
 
 namespace bfb {
@@ -32,13 +34,19 @@ constexpr float kGrow = 8.f;  // log2 of the growth that moves the maximum
 template <int DP>
 struct Layout {
   static constexpr int kStages = DP == 128 ? 4 : 6;
+  // With heads of up to 64 tensor memory has room for P beside S, and the next scores are made as soon as the
+  // softmax has read the last ones.  With 128 P lies over S, and the next scores wait for the product with P.
+  static constexpr bool kApart = DP == 64;
+  static constexpr int kO = 2 * kTile;                              // first column of the outputs
+  static constexpr int kP = kApart ? kO + 2 * DP : 0;               // of P of the first tile
+  static constexpr int kPStep = kApart ? kTile / 2 : kTile;         // from one tile's P to the other's
   static constexpr int kTileBytes = kTile * DP * 2;
   static constexpr int kPanel = kTile * 128;  // 64 columns of a tile
   static constexpr int kBytes = (2 + kStages) * kTileBytes + 1024;
 };
 
 struct Shared {
-  uint64_t q_full, kv_full[6], kv_empty[6], s_full[2], p_ready[2], grown[2], o_full[2], sums[2], tail, drained;
+  uint64_t q_full, kv_full[6], kv_empty[6], s_full[2], s_read[2], p_ready[2], pv_done[2], grown[2], o_full[2], sums[2], tail, drained;
   uint32_t tmem;
   int64_t q0, k0;
   int lq, lk, tile, part;
@@ -82,6 +90,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       for (int i = 0; i < 2; ++i) {
         bar_init(&s.s_full[i], 1);
+        bar_init(&s.s_read[i], 4);
+        bar_init(&s.pv_done[i], 1);
         bar_init(&s.p_ready[i], 8);  // a warp arrives once: 4 of softmax, 4 that scale O
         bar_init(&s.grown[i], 4);
         bar_init(&s.o_full[i], 1);
@@ -112,12 +122,15 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   if (warp < 8) {
     // ------------------------------------------------------------- softmax
-    regs_grow<200>();
+    regs_grow<184>();
     const int t = warp >> 2, row = threadIdx.x & (kTile - 1), steps = t ? n1 : n0;
-    const uint32_t ts = tmem + ((uint32_t)((warp & 3) * 32) << 16) + t * kTile;
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t ts = lanes + t * kTile, tp = lanes + L::kP + t * L::kPStep;
     const int i = (tile0 + t) * kTile + row, sees = seen(i);
     const int warp_sees = seen(i - lane);  // of the warp's first row: the fewest
-    const float c = a.scale * 1.4426950408889634f;
+    // positive: a negative scale's sign goes into the product, and 0 is the smallest number (hidden scores stay
+    // -inf, and every other exponent 0)
+    const float c = fmaxf(fabsf(a.scale) * 1.4426950408889634f, FLT_MIN);
     float top = -INFINITY, sum = 0.f;
     bool ok = true;
     for (int j = 0; j < steps && ok; ++j) {
@@ -128,25 +141,23 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int b = 0; b < 4; ++b) tmem_ld32(ts + 32 * b, x + 32 * b);
 #pragma unroll
       for (int b = 0; b < 4; ++b) tmem_ld_wait32(x + 32 * b);
-      const bool masked = (j + 1) * kTile > warp_sees;
-      const int limit = sees - j * kTile;
-      if (masked) {
+      if (L::kApart) {
+        tc_fence_before();
+        bar_arrive_warp(&s.s_read[t]);
+      }
+      if ((j + 1) * kTile > warp_sees) {  // some keys are hidden: their scores, whatever they are, become -inf
+        const int limit = sees - j * kTile;
 #pragma unroll
         for (int b = 0; b < kTile; ++b)
-          if (b >= limit) x[b] = 0xff800000u;  // -inf
+          if (b >= limit) x[b] = 0xff800000u;
       }
-      // largest of c S: of -|c| S where the scale is negative
       float best[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-      if (c >= 0.f) {
 #pragma unroll
-        for (int b = 0; b < kTile; ++b) best[b & 3] = fmaxf(best[b & 3], __uint_as_float(x[b]));
-      } else {
+      for (int b = 0; b < kTile; b += 8)
 #pragma unroll
-        for (int b = 0; b < kTile; ++b)
-          if (b < limit) best[b & 3] = fmaxf(best[b & 3], -__uint_as_float(x[b]));
-      }
-      float now = fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3])) * fabsf(c);
-      if (c == 0.f) now = limit > 0 ? 0.f : -INFINITY;
+        for (int e = 0; e < 4; ++e)
+          best[e] = fmaxf(best[e], fmaxf(__uint_as_float(x[b + 2 * e]), __uint_as_float(x[b + 2 * e + 1])));
+      const float now = fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3])) * c;
       float keep = 1.f;
       if (now > top + kGrow || top == -INFINITY) {
         keep = now == -INFINITY ? 1.f : exp2_approx(top - now);  // 0 at the first keys
@@ -157,6 +168,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float off = top == -INFINITY ? 0.f : -top;
       const float2 c2 = make_float2(c, c), off2 = make_float2(off, off);
       float2 part[2] = {};
+      if (L::kApart && j > 0) {  // P's columns are read
+        if (!(ok = bar_wait(&s.pv_done[t], (j - 1) & 1, &g_timeouts))) break;
+        tc_fence_after();
+      }
 #pragma unroll
       for (int b = 0; b < 4; ++b) {
         uint32_t p[16];
@@ -165,14 +180,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int at = 32 * b + 2 * e;
           float2 u = fma2(pair_of(x + at), c2, off2);
           u = make_float2(exp2_approx(u.x), exp2_approx(u.y));
-          if (masked) {
-            if (at >= limit) u.x = 0.f;
-            if (at + 1 >= limit) u.y = 0.f;
-          }
           part[e & 1] = add2(part[e & 1], u);
           p[e] = pack2<T>(u.x, u.y);
         }
-        tmem_st16(ts + 16 * b, p);
+        tmem_st16(tp + 16 * b, p);
       }
       part[0] = add2(part[0], part[1]);
       sum = sum * keep + (part[0].x + part[0].y);
@@ -186,17 +197,19 @@ __global__ void __launch_bounds__(kThreads, 1)
       a.lse[(int64_t)h * a.total_q + s.q0 + i] = sum == 0.f ? -INFINITY : (top + log2f(sum)) * 0.6931471805599453f;
   } else if (warp < 12) {
     // ------------------------------------------------- scaling O, the output
-    regs_shrink<64>();
+    regs_shrink<80>();
     const int row = threadIdx.x & (kTile - 1);
-    const uint32_t to = tmem + ((uint32_t)((warp & 3) * 32) << 16) + 2 * kTile;
+    const uint32_t to = tmem + ((uint32_t)((warp & 3) * 32) << 16) + L::kO;
     bool ok = true;
     for (int j = 0; j < n && ok; ++j) {
       for (int t = 0; t < 2; ++t) {
         if (j >= (t ? n1 : n0)) continue;
         if (!(ok = bar_wait(&s.grown[t], j & 1, &g_timeouts))) break;
         const float keep = s.scale[t][row];
-        // O holds the keys before: S of this step, which the softmax had, was issued behind their product
         if (j > 0 && __any_sync(0xffffffffu, keep != 1.f)) {
+          // O holds the keys before.  Where P lies over S that is known: the softmax has had this step's scores,
+          // which were issued behind their product.
+          if (L::kApart && !(ok = bar_wait(&s.pv_done[t], (j - 1) & 1, &g_timeouts))) break;
           tc_fence_after();
 #pragma unroll
           for (int b = 0; b < DP / 32; ++b) {
@@ -246,10 +259,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
     }
   } else {
-    regs_shrink<48>();
+    regs_shrink<64>();
     if (warp == 12 && n > 0) {
       // ---------------------------------------------------------- products
-      constexpr uint32_t ds = mma_desc(kBf16, kTile, false), dv = mma_desc(kBf16, DP, true);
+      constexpr uint32_t dv = mma_desc(kBf16, DP, true);
+      const uint32_t ds = mma_desc(kBf16, kTile, false) | (a.scale < 0.f ? kNegateA : 0u);
       const bool leader = elect_one();
       const uint32_t kv_addr = smem_u32(skv), q_addr = smem_u32(sq);
       auto score = [&](int t, int stage) {
@@ -281,13 +295,37 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (leader) mma_commit(&s.kv_empty[0]);
       }
       step();
+      auto output = [&](int t, int j, const TileDesc& vd, bool last) {
+        if (leader) {
+#pragma unroll
+          for (int c = 0; c < kTile / 16; ++c)
+            mma_ts(tmem + L::kO + t * DP, tmem + L::kP + t * L::kPStep + c * 8, vd.at(c * 2048), dv, j > 0 || c > 0);
+          if (L::kApart) mma_commit(&s.pv_done[t]);
+          if (last) mma_commit(&s.o_full[t]);
+        }
+      };
       for (int j = 0; j < n && ok; ++j) {
-        const int vs = stage;
+        const bool more = j + 1 < n;
+        int ks = 0, vs = 0;
+        if (L::kApart && more) {
+          ks = stage;
+          if (!(ok = full(stage, phase))) break;
+          step();
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (j + 1 >= (t ? n1 : n0)) continue;
+            if (!(ok = bar_wait(&s.s_read[t], j & 1, &g_timeouts))) break;
+            tc_fence_after();
+            score(t, ks);
+          }
+          if (!ok) break;
+          if (leader) mma_commit(&s.kv_empty[ks]);
+        }
+        vs = stage;
         if (!(ok = full(stage, phase))) break;
         step();
-        const int ks = stage;
-        const bool more = j + 1 < n;
-        if (more) {
+        if (!L::kApart && more) {
+          ks = stage;
           if (!(ok = full(stage, phase))) break;
           step();
         }
@@ -298,18 +336,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (j >= steps) continue;
           if (!(ok = bar_wait(&s.p_ready[t], j & 1, &g_timeouts))) break;
           tc_fence_after();
-          if (leader) {
-#pragma unroll
-            for (int c = 0; c < kTile / 16; ++c)
-              mma_ts(tmem + 2 * kTile + t * DP, tmem + t * kTile + c * 8, vd.at(c * 2048), dv, j > 0 || c > 0);
-          }
-          if (j + 1 < steps) score(t, ks);
-          else if (leader) mma_commit(&s.o_full[t]);
+          output(t, j, vd, j + 1 == steps);
+          if (!L::kApart && j + 1 < steps) score(t, ks);
         }
         if (!ok) break;
         if (leader) {
           mma_commit(&s.kv_empty[vs]);
-          if (more) mma_commit(&s.kv_empty[ks]);
+          if (!L::kApart && more) mma_commit(&s.kv_empty[ks]);
         }
       }
       // nothing leaves before its products are done
@@ -331,19 +364,22 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = true;
       int it = 0;
       for (; it < 2 * n; ++it) {
-        const int stage = it % L::kStages, j = it >> 1, valid = lk - j * kTile;
+        // in the order of their use: k0 v0 k1 v1 .., or k0 k1 v0 k2 v1 .. where the scores run ahead
+        const bool is_v = L::kApart ? it > 0 && (it % 2 == 0 || it == 2 * n - 1) : it % 2 == 1;
+        const int j = !L::kApart ? it >> 1 : it == 2 * n - 1 ? n - 1 : is_v ? it / 2 - 1 : (it + 1) / 2;
+        const int stage = it % L::kStages, valid = lk - j * kTile;
         if (lane == 0) ok = bar_wait(&s.kv_empty[stage], ((it / L::kStages) & 1) ^ 1, &g_timeouts);
         if (!(ok = __shfl_sync(0xffffffffu, ok, 0))) break;
         uint8_t* dst = skv + stage * L::kTileBytes;
         // Rows of v behind the last key are other sequences' (or anything): P is 0 there, but 0 * NaN is
         // not, so the last tile's are cleared before the product may read them.  k needs none of this:
         // its scores are replaced.
-        const bool clear = (it & 1) && valid < kTile;
+        const bool clear = is_v && valid < kTile;
         uint64_t* bar = clear ? &s.tail : &s.kv_full[stage];
         if (lane == 0) {
           bar_expect(bar, L::kTileBytes);
           for (int c = 0; c < DP / 64; ++c)
-            tma_load(dst + c * L::kPanel, (it & 1) ? &v_map : &k_map, 64 * c, m, (int)(k0 + (int64_t)j * kTile), bar);
+            tma_load(dst + c * L::kPanel, is_v ? &v_map : &k_map, 64 * c, m, (int)(k0 + (int64_t)j * kTile), bar);
         }
         if (clear) {  // once: the last tile
           ok = bar_wait(&s.tail, 0, &g_timeouts);

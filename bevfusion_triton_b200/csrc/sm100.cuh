@@ -119,6 +119,8 @@ __device__ __forceinline__ constexpr uint32_t mma_desc(bool bf16, int n, bool b_
          ((uint32_t)(n >> 3) << 17) | ((128u >> 4) << 24);
 }
 
+constexpr uint32_t kNegateA = 1u << 13;
+
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t desc, uint32_t accumulate) {
   asm volatile(
       "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(

@@ -40,25 +40,37 @@ __device__ __forceinline__ int64_t part_start(const int32_t* cu, int seqs, int64
   return cu ? min(max((int64_t)cu[i - 1], (int64_t)0), total) : 0;
 }
 
+// A tile of one part's queries (or keys), and the part's rows in both tensors.
 struct Tile {
   int part;        // -1: no such tile
-  int64_t start;   // first row of the part
-  int rows;        // rows of the part
-  int index;       // tile within the part
+  int index, tiles;  // the tile within the part, and how many it has
+  int64_t q0, k0;  // first rows
+  int lq, lk;      // queries, keys
+  int room;        // key rows, of which lk hold keys
 };
 
-// The item-th tile, found by one warp (all lanes take part and all get it).
-__device__ __forceinline__ Tile find_tile(const int32_t* cu, int seqs, int64_t total, int rows, int64_t item) {
+// The item-th tile of `rows` rows of the queries (or keys), found by one warp:
+// all lanes take part and all get it.
+template <bool kKeys>
+__device__ __forceinline__ Tile find_tile(const Args& a, int rows, int64_t item) {
   const int lane = threadIdx.x & 31;
   int64_t before = 0;
-  for (int base = 0; base < seqs + 2; base += 32) {
+  for (int base = 0; base < a.seqs + 2; base += 32) {
     const int part = base + lane;
-    int64_t start = 0, n = 0;
-    if (part < seqs + 2) {
-      start = part_start(cu, seqs, total, part);
-      n = max(part_start(cu, seqs, total, part + 1) - start, (int64_t)0);
+    int64_t q0 = 0, k0 = 0;
+    int lq = 0, room = 0, lk = 0;
+    if (part < a.seqs + 2) {  // all loads at once: one latency
+      const bool seq = part >= 1 && part <= a.seqs;
+      const int used = seq && a.kv_lengths ? a.kv_lengths[part - 1] : 0x7fffffff;
+      q0 = part_start(a.cu_q, a.seqs, a.total_q, part);
+      k0 = part_start(a.cu_k, a.seqs, a.total_k, part);
+      const int64_t q1 = part_start(a.cu_q, a.seqs, a.total_q, part + 1);
+      const int64_t k1 = part_start(a.cu_k, a.seqs, a.total_k, part + 1);
+      lq = (int)max(q1 - q0, (int64_t)0);
+      room = (int)max(k1 - k0, (int64_t)0);
+      lk = seq ? min(max(used, 0), room) : 0;
     }
-    const int64_t tiles = (n + rows - 1) / rows;
+    const int tiles = ((kKeys ? room : lq) + rows - 1) / rows;
     int64_t upto = tiles;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -70,29 +82,25 @@ __device__ __forceinline__ Tile find_tile(const int32_t* cu, int seqs, int64_t t
       const int src = __ffs(hit) - 1;
       Tile t;
       t.part = base + src;
-      t.start = __shfl_sync(0xffffffffu, start, src);
-      t.rows = (int)__shfl_sync(0xffffffffu, n, src);
-      t.index = (int)(item - before - __shfl_sync(0xffffffffu, upto - tiles, src));
+      t.tiles = __shfl_sync(0xffffffffu, tiles, src);
+      t.index = (int)(item - before - __shfl_sync(0xffffffffu, upto, src)) + t.tiles;
+      t.q0 = __shfl_sync(0xffffffffu, q0, src);
+      t.k0 = __shfl_sync(0xffffffffu, k0, src);
+      t.lq = __shfl_sync(0xffffffffu, lq, src);
+      t.lk = __shfl_sync(0xffffffffu, lk, src);
+      t.room = __shfl_sync(0xffffffffu, room, src);
+      // the rows of no sequence have nothing in the other tensor
+      if (t.part < 1 || t.part > a.seqs) {
+        if (kKeys) t.lq = 0;
+        t.lk = 0;
+      }
       return t;
     }
     before += __shfl_sync(0xffffffffu, upto, 31);
   }
-  return {-1, 0, 0, 0};
-}
-
-// Rows of part `part` in the other tensor of the pair (none for the parts
-// that are no sequence).
-__device__ __forceinline__ void other_rows(const int32_t* cu, int seqs, int64_t total, int part, int64_t& start,
-                                           int& rows) {
-  start = 0;
-  rows = 0;
-  if (part < 1 || part > seqs) return;
-  start = part_start(cu, seqs, total, part);
-  rows = (int)max(part_start(cu, seqs, total, part + 1) - start, (int64_t)0);
-}
-
-__device__ __forceinline__ int used_keys(const int32_t* kv_lengths, int part, int rows) {
-  return kv_lengths && rows > 0 ? min(max(kv_lengths[part - 1], 0), rows) : rows;
+  Tile none = {};
+  none.part = -1;
+  return none;
 }
 
 // Tensor map of [rows, heads, dim] 16-bit values whose box is 128 rows of 64

@@ -51,8 +51,7 @@ struct Shared {
   uint64_t own_full, a_full[kFirst], a_empty[kFirst], b_full[kSecond], b_empty[kSecond];
   uint64_t s_full, dp_full, p_ready, ds_ready, done, tail;
   uint32_t tmem;
-  int part, tile, lq, lk, room;
-  int64_t q0, k0;
+  Tile tile;
   float lse2[kFirst][kTile], delta[kSecond][kTile];  // dQ: delta's first half row from each warpgroup
 };
 
@@ -145,31 +144,11 @@ __device__ __forceinline__ void write_row(uint32_t from, T* out, int col0, int c
 template <bool kKeys>
 __device__ __forceinline__ bool setup(Shared& s, const Args& a, int64_t item) {
   if (threadIdx.x < 32) {
-    const Tile t = kKeys ? find_tile(a.cu_k, a.seqs, a.total_k, kTile, item)
-                         : find_tile(a.cu_q, a.seqs, a.total_q, kTile, item);
+    Tile t = find_tile<kKeys>(a, kTile, item);
+    // causal: the last query tiles, which see the most keys, start first
+    if (!kKeys) t.index = t.tiles - 1 - t.index;
     if (threadIdx.x == 0) {
-      s.part = t.part;
-      if (t.part >= 0) {
-        int64_t start;
-        int rows;
-        if (kKeys) {
-          other_rows(a.cu_q, a.seqs, a.total_q, t.part, start, rows);
-          s.k0 = t.start;
-          s.room = t.rows;
-          s.q0 = start;
-          s.lq = rows;
-          s.lk = t.part >= 1 && t.part <= a.seqs ? used_keys(a.kv_lengths, t.part, t.rows) : 0;
-          s.tile = t.index;
-        } else {
-          other_rows(a.cu_k, a.seqs, a.total_k, t.part, start, rows);
-          s.q0 = t.start;
-          s.lq = t.rows;
-          s.k0 = start;
-          s.lk = used_keys(a.kv_lengths, t.part, rows);
-          // causal: the last tiles, which see the most keys, start first
-          s.tile = (t.rows + kTile - 1) / kTile - 1 - t.index;
-        }
-      }
+      s.tile = t;
       bar_init(&s.own_full, 1);
       for (int i = 0; i < kFirst; ++i) {
         bar_init(&s.a_full[i], 2);
@@ -189,7 +168,7 @@ __device__ __forceinline__ bool setup(Shared& s, const Args& a, int64_t item) {
     }
   }
   __syncthreads();
-  return s.part >= 0;
+  return s.tile.part >= 0;
 }
 
 __device__ __forceinline__ uint32_t tmem_start(Shared& s, int warp) {
@@ -284,7 +263,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (!setup<true>(s, a, blockIdx.x / a.kv_heads)) return;
   const uint32_t tmem = tmem_start(s, warp);
   const uint32_t ts = tmem, tdp = tmem + kTile, tdv = tmem + 2 * kTile, tdk = tdv + DP;
-  const int lq = s.lq, lk = s.lk, j0 = s.tile * kTile, shift = lk - lq;
+  const Tile place = s.tile;
+  const int lq = place.lq, lk = place.lk, j0 = place.index * kTile, shift = lk - lq;
   // query tiles that see any of these keys: from the one with the first row i that has i + shift >= j0
   const int first = a.causal ? max(0, j0 - shift) / kTile : 0;
   const int per_head = j0 < lk ? max(0, (lq + kTile - 1) / kTile - first) : 0;
@@ -373,8 +353,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (ok && (n == 0 || bar_wait(&s.done, 0, &g_timeouts))) {
       tc_fence_after();
-      T* out = static_cast<T*>(wg ? a.dk : a.dv) + ((s.k0 + j) * a.kv_heads + m) * a.dim;
-      write_row<T>((wg ? tdk : tdv) + lanes, out, 0, DP, a.dim, j < s.room, n == 0 || j >= lk);
+      T* out = static_cast<T*>(wg ? a.dk : a.dv) + ((place.k0 + j) * a.kv_heads + m) * a.dim;
+      write_row<T>((wg ? tdk : tdv) + lanes, out, 0, DP, a.dim, j < place.room, n == 0 || j >= lk);
     }
   } else {
     regs_shrink<88>();
@@ -424,20 +404,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (warp == 9 && n > 0) {
       if (lane == 0) {
         bar_expect(&s.own_full, 2 * L::kTileBytes);
-        load_tile<DP>(sk, &k_map, m, s.k0 + j0, &s.own_full);
-        load_tile<DP>(sv, &v_map, m, s.k0 + j0, &s.own_full);
+        load_tile<DP>(sk, &k_map, m, place.k0 + j0, &s.own_full);
+        load_tile<DP>(sv, &v_map, m, place.k0 + j0, &s.own_full);
       }
       uint32_t tails = 0;
       int i = 0, a_loads = 0, tile = 0, h = m * group;
       for (; i < n; ++i) {
         const int q = (first + tile) * kTile, valid = lq - q, sa = i % kFirst, sb = i % kSecond;
-        const int64_t at = (int64_t)h * a.total_q + s.q0 + q;
+        const int64_t at = (int64_t)h * a.total_q + place.q0 + q;
         // rows past the sequence: P = exp2(-inf) = 0
-        if (!load_stage<DP, true>(sq + sa * L::kTileBytes, &q_map, h, s.q0 + q, valid, &s.a_full[sa], &s.a_empty[sa],
+        if (!load_stage<DP, true>(sq + sa * L::kTileBytes, &q_map, h, place.q0 + q, valid, &s.a_full[sa], &s.a_empty[sa],
                                   (i / kFirst) & 1, &s.tail, tails, a.lse2 + at, s.lse2[sa], -INFINITY))
           break;
         ++a_loads;
-        if (!load_stage<DP, true>(sg + sb * L::kTileBytes, &g_map, h, s.q0 + q, valid, &s.b_full[sb], &s.b_empty[sb],
+        if (!load_stage<DP, true>(sg + sb * L::kTileBytes, &g_map, h, place.q0 + q, valid, &s.b_full[sb], &s.b_empty[sb],
                                   (i / kSecond) & 1, &s.tail, tails, a.delta + at, s.delta[sb], 0.f))
           break;
         if (++tile == per_head) {
@@ -470,7 +450,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (!setup<false>(s, a, blockIdx.x / a.heads)) return;
   const uint32_t tmem = tmem_start(s, warp);
   const uint32_t ts = tmem, tdp = tmem + kTile, tdq = tmem + 2 * kTile;
-  const int lq = s.lq, lk = s.lk, i0 = s.tile * kTile, shift = lk - lq;
+  const Tile place = s.tile;
+  const int lq = place.lq, lk = place.lk, i0 = place.index * kTile, shift = lk - lq;
   auto seen = [&](int i) { return a.causal ? max(0, min(lk, i + shift + 1)) : lk; };
   const int n = (seen(min(lq, i0 + kTile) - 1) + kTile - 1) / kTile;
 
@@ -479,7 +460,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int wg = warp >> 2, row = threadIdx.x & (kTile - 1), i = i0 + row;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, mine = lanes + wg * kHalf;
     const float2 c2 = make_float2(a.scale * kLog2e, a.scale * kLog2e), scale2 = make_float2(a.scale, a.scale);
-    const int64_t at = (int64_t)h * a.total_q + s.q0 + i;
+    const int64_t at = (int64_t)h * a.total_q + place.q0 + i;
     const float lse2 = i < lq ? a.lse2[at] : INFINITY;
     const bool exact = lk <= kTile;  // one tile of keys: delta is summed here
     float delta = i < lq && !exact ? a.delta[at] : 0.f;
@@ -543,7 +524,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (ok && (n == 0 || bar_wait(&s.done, 0, &g_timeouts))) {
       tc_fence_after();
-      T* out = static_cast<T*>(a.dq) + ((s.q0 + i) * a.heads + h) * a.dim;
+      T* out = static_cast<T*>(a.dq) + ((place.q0 + i) * a.heads + h) * a.dim;
       write_row<T>(tdq + lanes + wg * (DP / 2), out, wg * (DP / 2), DP / 2, a.dim, i < lq, n == 0);
     }
   } else {
@@ -595,14 +576,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     } else if (warp == 9 && n > 0) {
       if (lane == 0) {
         bar_expect(&s.own_full, 2 * L::kTileBytes);
-        load_tile<DP>(sq, &q_map, h, s.q0 + i0, &s.own_full);
-        load_tile<DP>(sg, &g_map, h, s.q0 + i0, &s.own_full);
+        load_tile<DP>(sq, &q_map, h, place.q0 + i0, &s.own_full);
+        load_tile<DP>(sg, &g_map, h, place.q0 + i0, &s.own_full);
       }
       uint32_t tails = 0;
       int j = 0, a_loads = 0;
       for (; j < n; ++j) {
         const int valid = lk - j * kTile, sa = j % kFirst, sb = j % kSecond;
-        const int64_t k = s.k0 + (int64_t)j * kTile;
+        const int64_t k = place.k0 + (int64_t)j * kTile;
         if (!load_stage<DP, true>(sk + sa * L::kTileBytes, &k_map, m, k, valid, &s.a_full[sa], &s.a_empty[sa],
                                   (j / kFirst) & 1, &s.tail, tails))
           break;

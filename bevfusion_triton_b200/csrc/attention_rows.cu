@@ -54,7 +54,7 @@ __device__ __forceinline__ Seq seq_at(const Args& a, int s) {
   x.lq = (int)max(part_start(a.cu_q, a.seqs, a.total_q, s + 2) - x.q0, (int64_t)0);
   x.k0 = part_start(a.cu_k, a.seqs, a.total_k, s + 1);
   const int room = (int)max(part_start(a.cu_k, a.seqs, a.total_k, s + 2) - x.k0, (int64_t)0);
-  x.lk = used_keys(a.kv_lengths, s + 1, room);
+  x.lk = a.kv_lengths ? min(max(a.kv_lengths[s], 0), room) : room;
   x.row_tiles = (int)(((int64_t)x.lq * (a.heads / a.kv_heads) + kRows - 1) / kRows);
   x.tiles = (x.lk + kKeys - 1) / kKeys;
   x.work = (int64_t)x.row_tiles * x.tiles * a.kv_heads;

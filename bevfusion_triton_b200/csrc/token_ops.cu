@@ -37,6 +37,7 @@ constexpr int kMostPartials = 148 * 4 + kMostShares;
 // Dynamic shared memory of a block: 256 rows' sums of 16 columns each, or the angles of up to 4 x 256 tokens of 16
 // values (one lane a row): the rows of a step hold 16 * kThreads values at most.
 constexpr int kMostAngles = 4 * kThreads * 16 * 4;
+constexpr size_t kPlainSmem = 32 << 10;  // up to here (beside the static tables) no kernel has to ask
 
 // 8 consecutive values as they lie in memory (16-byte aligned).
 template <class T>
@@ -750,7 +751,7 @@ extern "C" int bfb_qk_norm_rotary(const void* q_dev, const void* k_dev, int64_t 
                 : dtype == BFB_F16 ? (interleaved ? rotary_forward_kernel<__half, true> : rotary_forward_kernel<__half, false>)
                                    : (interleaved ? rotary_forward_kernel<__nv_bfloat16, true>
                                                   : rotary_forward_kernel<__nv_bfloat16, false>);
-  BFB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostAngles));
+  if (smem > kPlainSmem) BFB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostAngles));
   kernel<<<dim3(g.x, g.y), g.threads, smem, as_stream(stream)>>>(a);
   BFB_CHECK_LAUNCH();
   return BFB_OK;
@@ -797,7 +798,7 @@ extern "C" int bfb_qk_norm_rotary_backward(
                   : dtype == BFB_F16 ? (interleaved ? rotary_backward_kernel<__half, true> : rotary_backward_kernel<__half, false>)
                                      : (interleaved ? rotary_backward_kernel<__nv_bfloat16, true>
                                                     : rotary_backward_kernel<__nv_bfloat16, false>);
-    BFB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostAngles));
+    if (smem > kPlainSmem) BFB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMostAngles));
     kernel<<<dim3(g.x, g.y), g.threads, smem, as_stream(stream)>>>(a);
     BFB_CHECK_LAUNCH();
   }

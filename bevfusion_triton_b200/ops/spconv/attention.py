@@ -26,6 +26,17 @@ from .modules import SparseModule
 from .ops import _require_cuda
 from .structure import SparseConvTensor
 
+_handles = None
+
+
+def _native():
+    """The three operators, looked up once: a call is short enough for the look-up to show."""
+    global _handles
+    if _handles is None:
+        o = ops()
+        _handles = (o.packed_attention.default, o.qk_norm_rotary.default, o.residual_dropout.default)
+    return _handles
+
 
 def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens_q: torch.Tensor,
                      cu_seqlens_k: torch.Tensor | None = None, kv_lengths: torch.Tensor | None = None,
@@ -60,8 +71,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
         dt = torch.get_autocast_dtype('cuda')
         back = None if q.dtype == dt else q.dtype
         q, k, v = q.to(dt), k.to(dt), v.to(dt)
-    out, lse = ops().packed_attention(q, k, v, cu_seqlens_q, cu_seqlens_q if cu_seqlens_k is None else cu_seqlens_k,
-                                      kv_lengths, bool(causal), float(scale))
+    out, lse = _native()[0](q, k, v, cu_seqlens_q, cu_seqlens_q if cu_seqlens_k is None else cu_seqlens_k, kv_lengths,
+                             bool(causal), float(scale))
     if back is not None:
         out = out.to(back)
     return (out, lse) if return_lse else out
@@ -89,7 +100,7 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, in
         q_weight = q_weight.float()
     if k_weight is not None and k_weight.dtype != torch.float32:
         k_weight = k_weight.float()
-    return ops().qk_norm_rotary(q, k, positions, inv_freq, sections, q_weight, k_weight, eps, bool(interleaved))
+    return _native()[1](q, k, positions, inv_freq, sections, q_weight, k_weight, eps, bool(interleaved))
 
 
 def residual_dropout(x: torch.Tensor, residual: torch.Tensor | None, p: float, seed: torch.Tensor) -> torch.Tensor:
@@ -103,7 +114,7 @@ def residual_dropout(x: torch.Tensor, residual: torch.Tensor | None, p: float, s
     seed's values are changed between replays.  0 <= p <= 1.
     """
     _require_cuda(x, seed)
-    return ops().residual_dropout(x, residual, p, seed)
+    return _native()[2](x, residual, p, seed)
 
 
 def sample_offsets(indices: torch.Tensor, batch_size: int) -> torch.Tensor:

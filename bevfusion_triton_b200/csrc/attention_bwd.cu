@@ -39,6 +39,9 @@ template <int DP>
 struct Layout {
   static constexpr int kTileBytes = kTile * DP * 2;
   static constexpr int kPanel = kTile * 128;
+  // dV's product starts on the first half of P while the second is formed: with heads of 128, where a product takes
+  // as long as that (causal, 0.7 - 4 k tokens, 16/4 heads: 295 -> 285 us; with 64 the arrivals cost more, 83 -> 85)
+  static constexpr bool kSplit = DP == 128;
   static constexpr int kTiles = 7;  // two resident tiles, three of the first ring, two of the second
 };
 
@@ -49,10 +52,11 @@ constexpr int kFirst = 3, kSecond = 2;
 
 struct Shared {
   uint64_t own_full, a_full[kFirst], a_empty[kFirst], b_full[kSecond], b_empty[kSecond];
-  uint64_t s_full, dp_full, p_ready, ds_ready, done, tail;
+  uint64_t s_full, dp_full, p_half, p_ready, ds_ready, halves, done, tail;
   uint32_t tmem;
   Tile tile;
-  float lse2[kFirst][kTile], delta[kSecond][kTile];  // dQ: delta's first half row from each warpgroup
+  alignas(16) float lse2[kFirst][kTile];  // read four at a time
+  alignas(16) float delta[kSecond][kTile];  // dQ: delta's first half row from each warpgroup
 };
 
 template <int DP>
@@ -81,19 +85,32 @@ __device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* map, 
 
 // dst += A B over 128 rows of B (A in tensor memory, B's rows along K).
 template <int DP, bool kBf16>
-__device__ __forceinline__ void product_rows(bool leader, uint32_t dst, uint32_t a, uint32_t b, bool first) {
+__device__ __forceinline__ void product_rows(uint32_t dst, uint32_t a, uint32_t b, bool first) {
   const TileDesc bd(b, Layout<DP>::kPanel);
-  if (leader) {
+  if (elect_one()) {
 #pragma unroll
     for (int c = 0; c < kTile / 16; ++c)
       mma_ts(dst, a + half_step(c), bd.at(c * 2048), mma_desc(kBf16, DP, true), !first || c > 0);
   }
 }
+// The half of its steps whose columns each warpgroup wrote first (c0 = 0) or last (2).
+template <int DP, bool kBf16>
+__device__ __forceinline__ void product_rows_half(uint32_t dst, uint32_t a, uint32_t b, bool first,
+                                                  int c0) {
+  const TileDesc bd(b, Layout<DP>::kPanel);
+  if (elect_one()) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int c = c0 + (e & 1) + (e >> 1) * 4;
+      mma_ts(dst, a + half_step(c), bd.at(c * 2048), mma_desc(kBf16, DP, true), !first || e > 0);
+    }
+  }
+}
 // dst = A B^T over the columns of two tiles.
 template <int DP, bool kBf16>
-__device__ __forceinline__ void product_cols(bool leader, uint32_t dst, uint32_t a, uint32_t b) {
+__device__ __forceinline__ void product_cols(uint32_t dst, uint32_t a, uint32_t b) {
   const TileDesc ad(a, 16), bd(b, 16);
-  if (leader) {
+  if (elect_one()) {
 #pragma unroll
     for (int c = 0; c < DP / 16; ++c) {
       const uint32_t off = (c / 4) * Layout<DP>::kPanel + (c % 4) * 32;
@@ -144,9 +161,7 @@ __device__ __forceinline__ void write_row(uint32_t from, T* out, int col0, int c
 template <bool kKeys>
 __device__ __forceinline__ bool setup(Shared& s, const Args& a, int64_t item) {
   if (threadIdx.x < 32) {
-    Tile t = find_tile<kKeys>(a, kTile, item);
-    // causal: the last query tiles, which see the most keys, start first
-    if (!kKeys) t.index = t.tiles - 1 - t.index;
+    const Tile t = find_tile<kKeys>(a, kTile, item);
     if (threadIdx.x == 0) {
       s.tile = t;
       bar_init(&s.own_full, 1);
@@ -160,8 +175,10 @@ __device__ __forceinline__ bool setup(Shared& s, const Args& a, int64_t item) {
       }
       bar_init(&s.s_full, 1);
       bar_init(&s.dp_full, 1);
+      bar_init(&s.p_half, 8);
       bar_init(&s.p_ready, 8);  // one arrival of each warp
       bar_init(&s.ds_ready, 8);
+      bar_init(&s.halves, 8);
       bar_init(&s.done, 1);
       bar_init(&s.tail, 1);
       fence_bar_init();
@@ -217,7 +234,7 @@ __device__ __forceinline__ bool load_stage(uint8_t* dst, const CUtensorMap* map,
     for (int e = 0; e < 4; ++e) values[lane + 32 * e] = x[e];
   }
   if (clear) {
-    ok = bar_wait(tail, tails & 1, &g_timeouts);
+    ok = bar_wait_warp(tail, tails & 1, &g_timeouts);
     ++tails;
     if (!__all_sync(0xffffffffu, ok)) return false;
     clear_rows<DP>(dst, valid);
@@ -279,7 +296,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     int tile = 0;
     for (int i = 0; i < n; ++i) {
       const int sa = i % kFirst, sb = i % kSecond;
-      if (!(ok = bar_wait(&s.a_full[sa], (i / kFirst) & 1, &g_timeouts) && bar_wait(&s.s_full, i & 1, &g_timeouts)))
+      if (!(ok = bar_wait_warp(&s.a_full[sa], (i / kFirst) & 1, &g_timeouts) && bar_wait_warp(&s.s_full, i & 1, &g_timeouts)))
         break;
       tc_fence_after();
       uint32_t x[kHalf];
@@ -304,23 +321,25 @@ __global__ void __launch_bounds__(kThreads, 1)
         p[e + 1] = exp2_approx(u.y);
         p[e + 2] = exp2_approx(v.x);
         p[e + 3] = exp2_approx(v.y);
-      }
-      if (masked) {
+        if (e % 32 == 28) {
+          const int b = e / 32;
+          if (masked) {
 #pragma unroll
-        for (int e = 0; e < kHalf; ++e)
-          if (e < from) p[e] = 0.f;
-      }
+            for (int f = 32 * b; f < 32 * b + 32; ++f)
+              if (f < from) p[f] = 0.f;
+          }
+          uint32_t w[16];
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        uint32_t w[16];
-#pragma unroll
-        for (int e = 0; e < 16; ++e) w[e] = pack2<T>(p[32 * b + 2 * e], p[32 * b + 2 * e + 1]);
-        tmem_st16(ts + mine + 16 * b, w);
+          for (int f = 0; f < 16; ++f) w[f] = pack2<T>(p[32 * b + 2 * f], p[32 * b + 2 * f + 1]);
+          tmem_st16(ts + mine + 16 * b, w);
+          if (b == 1 || L::kSplit) {
+            tmem_st_wait();
+            tc_fence_before();
+            bar_arrive_warp(b ? &s.p_ready : &s.p_half);
+          }
+        }
       }
-      tmem_st_wait();
-      tc_fence_before();
-      bar_arrive_warp(&s.p_ready);
-      if (!(ok = bar_wait(&s.b_full[sb], (i / kSecond) & 1, &g_timeouts) && bar_wait(&s.dp_full, i & 1, &g_timeouts)))
+      if (!(ok = bar_wait_warp(&s.b_full[sb], (i / kSecond) & 1, &g_timeouts) && bar_wait_warp(&s.dp_full, i & 1, &g_timeouts)))
         break;
       tc_fence_after();
       tmem_ld32(tdp + mine, x);
@@ -351,7 +370,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_before();
       bar_arrive_warp(&s.ds_ready);
     }
-    if (ok && (n == 0 || bar_wait(&s.done, 0, &g_timeouts))) {
+    if (ok && (n == 0 || bar_wait_warp(&s.done, 0, &g_timeouts))) {
       tc_fence_after();
       T* out = static_cast<T*>(wg ? a.dk : a.dv) + ((place.k0 + j) * a.kv_heads + m) * a.dim;
       write_row<T>((wg ? tdk : tdv) + lanes, out, 0, DP, a.dim, j < place.room, n == 0 || j >= lk);
@@ -359,18 +378,17 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     regs_shrink<88>();
     if (warp == 8 && n > 0) {
-      const bool leader = elect_one();
       const uint32_t ka = smem_u32(sk), va = smem_u32(sv), q_addr = smem_u32(sq), g_addr = smem_u32(sg);
       Ring<kFirst> qr;  // of the next scores
       Ring<kSecond> gr;
-      bool ok = bar_wait(&s.own_full, 0, &g_timeouts) && bar_wait(&s.a_full[0], 0, &g_timeouts) &&
-                bar_wait(&s.b_full[0], 0, &g_timeouts);
+      bool ok = bar_wait_warp(&s.own_full, 0, &g_timeouts) && bar_wait_warp(&s.a_full[0], 0, &g_timeouts) &&
+                bar_wait_warp(&s.b_full[0], 0, &g_timeouts);
       if (ok) {
         tc_fence_after();
-        product_cols<DP, kBf16>(leader, ts, ka, q_addr);
-        if (leader) mma_commit(&s.s_full);
-        product_cols<DP, kBf16>(leader, tdp, va, g_addr);
-        if (leader) mma_commit(&s.dp_full);
+        product_cols<DP, kBf16>(ts, ka, q_addr);
+        if (elect_one()) mma_commit(&s.s_full);
+        product_cols<DP, kBf16>(tdp, va, g_addr);
+        if (elect_one()) mma_commit(&s.dp_full);
       }
       for (int i = 0; i < n && ok; ++i) {
         const bool more = i + 1 < n;
@@ -378,29 +396,38 @@ __global__ void __launch_bounds__(kThreads, 1)
         const uint32_t q_now = q_addr + qs * L::kTileBytes, g_now = g_addr + gs * L::kTileBytes;
         qr.step();
         gr.step();
-        if (!(ok = bar_wait(&s.p_ready, i & 1, &g_timeouts))) break;
-        tc_fence_after();
-        product_rows<DP, kBf16>(leader, tdv, ts, g_now, i == 0);
-        if (more) {
-          if (!(ok = bar_wait(&s.a_full[qr.stage], qr.phase, &g_timeouts))) break;
-          product_cols<DP, kBf16>(leader, ts, ka, q_addr + qr.stage * L::kTileBytes);
-          if (leader) mma_commit(&s.s_full);
+        if (L::kSplit) {
+          if (!(ok = bar_wait_warp(&s.p_half, i & 1, &g_timeouts))) break;
+          tc_fence_after();
+          product_rows_half<DP, kBf16>(tdv, ts, g_now, i == 0, 0);
+          if (!(ok = bar_wait_warp(&s.p_ready, i & 1, &g_timeouts))) break;
+          tc_fence_after();
+          product_rows_half<DP, kBf16>(tdv, ts, g_now, false, 2);
+        } else {
+          if (!(ok = bar_wait_warp(&s.p_ready, i & 1, &g_timeouts))) break;
+          tc_fence_after();
+          product_rows<DP, kBf16>(tdv, ts, g_now, i == 0);
         }
-        if (!(ok = bar_wait(&s.ds_ready, i & 1, &g_timeouts))) break;
+        if (more) {
+          if (!(ok = bar_wait_warp(&s.a_full[qr.stage], qr.phase, &g_timeouts))) break;
+          product_cols<DP, kBf16>(ts, ka, q_addr + qr.stage * L::kTileBytes);
+          if (elect_one()) mma_commit(&s.s_full);
+        }
+        if (!(ok = bar_wait_warp(&s.ds_ready, i & 1, &g_timeouts))) break;
         tc_fence_after();
-        product_rows<DP, kBf16>(leader, tdk, tdp, q_now, i == 0);
-        if (leader) {  // both: the threads are done with lse2 and delta, too
+        product_rows<DP, kBf16>(tdk, tdp, q_now, i == 0);
+        if (elect_one()) {  // both: the threads are done with lse2 and delta, too
           mma_commit(&s.a_empty[qs]);
           mma_commit(&s.b_empty[gs]);
         }
         if (more) {
-          if (!(ok = bar_wait(&s.b_full[gr.stage], gr.phase, &g_timeouts))) break;
-          product_cols<DP, kBf16>(leader, tdp, va, g_addr + gr.stage * L::kTileBytes);
-          if (leader) mma_commit(&s.dp_full);
+          if (!(ok = bar_wait_warp(&s.b_full[gr.stage], gr.phase, &g_timeouts))) break;
+          product_cols<DP, kBf16>(tdp, va, g_addr + gr.stage * L::kTileBytes);
+          if (elect_one()) mma_commit(&s.dp_full);
         }
       }
-      if (leader) mma_commit(&s.done);
-      bar_wait(&s.done, 0, &g_timeouts);  // nothing leaves before its products are done
+      if (elect_one()) mma_commit(&s.done);
+      bar_wait_warp(&s.done, 0, &g_timeouts);  // nothing leaves before its products are done
     } else if (warp == 9 && n > 0) {
       if (lane == 0) {
         bar_expect(&s.own_full, 2 * L::kTileBytes);
@@ -467,7 +494,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int sees = seen(i), warp_sees = seen(i - lane);
     bool ok = true;
     for (int j = 0; j < n; ++j) {
-      if (!(ok = bar_wait(&s.s_full, j & 1, &g_timeouts))) break;
+      if (!(ok = bar_wait_warp(&s.s_full, j & 1, &g_timeouts))) break;
       tc_fence_after();
       uint32_t x[kHalf];
       tmem_ld32(ts + mine, x);
@@ -485,7 +512,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         p[e] = exp2_approx(u.x);
         p[e + 1] = exp2_approx(u.y);
       }
-      if (!(ok = bar_wait(&s.dp_full, j & 1, &g_timeouts))) break;
+      if (!(ok = bar_wait_warp(&s.dp_full, j & 1, &g_timeouts))) break;
       tc_fence_after();
       tmem_ld32(tdp + mine, x);
       tmem_ld32(tdp + mine + 32, x + 32);
@@ -496,7 +523,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int e = 0; e < kHalf; ++e) part += e < limit ? p[e] * __uint_as_float(x[e]) : 0.f;
         s.delta[wg][row] = part;
-        asm volatile("bar.sync 1, 256;" ::: "memory");  // the two warpgroups
+        bar_arrive_warp(&s.halves);  // the two warpgroups; once, as there is one tile
+        if (!(ok = bar_wait_warp(&s.halves, 0, &g_timeouts))) break;
         if (i < lq) {
           delta = a.scale * (s.delta[0][row] + s.delta[1][row] - (a.dlse ? a.dlse[at] : 0.f));
           if (wg == 0) a.delta[at] = delta;
@@ -522,7 +550,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_before();
       bar_arrive_warp(&s.ds_ready);
     }
-    if (ok && (n == 0 || bar_wait(&s.done, 0, &g_timeouts))) {
+    if (ok && (n == 0 || bar_wait_warp(&s.done, 0, &g_timeouts))) {
       tc_fence_after();
       T* out = static_cast<T*>(a.dq) + ((place.q0 + i) * a.heads + h) * a.dim;
       write_row<T>(tdq + lanes + wg * (DP / 2), out, wg * (DP / 2), DP / 2, a.dim, i < lq, n == 0);
@@ -530,18 +558,17 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     regs_shrink<88>();
     if (warp == 8 && n > 0) {
-      const bool leader = elect_one();
       const uint32_t qa = smem_u32(sq), ga = smem_u32(sg), k_addr = smem_u32(sk), v_addr = smem_u32(sv);
       Ring<kFirst> kr;  // of the next scores
       Ring<kSecond> vr;
-      bool ok = bar_wait(&s.own_full, 0, &g_timeouts) && bar_wait(&s.a_full[0], 0, &g_timeouts) &&
-                bar_wait(&s.b_full[0], 0, &g_timeouts);
+      bool ok = bar_wait_warp(&s.own_full, 0, &g_timeouts) && bar_wait_warp(&s.a_full[0], 0, &g_timeouts) &&
+                bar_wait_warp(&s.b_full[0], 0, &g_timeouts);
       if (ok) {
         tc_fence_after();
-        product_cols<DP, kBf16>(leader, ts, qa, k_addr);
-        if (leader) mma_commit(&s.s_full);
-        product_cols<DP, kBf16>(leader, tdp, ga, v_addr);
-        if (leader) {
+        product_cols<DP, kBf16>(ts, qa, k_addr);
+        if (elect_one()) mma_commit(&s.s_full);
+        product_cols<DP, kBf16>(tdp, ga, v_addr);
+        if (elect_one()) {
           mma_commit(&s.dp_full);
           mma_commit(&s.b_empty[0]);
         }
@@ -551,28 +578,28 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int ks = kr.stage;
         kr.step();
         vr.step();
-        if (!(ok = bar_wait(&s.p_ready, j & 1, &g_timeouts))) break;
+        if (!(ok = bar_wait_warp(&s.p_ready, j & 1, &g_timeouts))) break;
         tc_fence_after();
         if (more) {
-          if (!(ok = bar_wait(&s.a_full[kr.stage], kr.phase, &g_timeouts))) break;
-          product_cols<DP, kBf16>(leader, ts, qa, k_addr + kr.stage * L::kTileBytes);
-          if (leader) mma_commit(&s.s_full);
+          if (!(ok = bar_wait_warp(&s.a_full[kr.stage], kr.phase, &g_timeouts))) break;
+          product_cols<DP, kBf16>(ts, qa, k_addr + kr.stage * L::kTileBytes);
+          if (elect_one()) mma_commit(&s.s_full);
         }
-        if (!(ok = bar_wait(&s.ds_ready, j & 1, &g_timeouts))) break;
+        if (!(ok = bar_wait_warp(&s.ds_ready, j & 1, &g_timeouts))) break;
         tc_fence_after();
-        product_rows<DP, kBf16>(leader, tdq, tdp, k_addr + ks * L::kTileBytes, j == 0);
-        if (leader) mma_commit(&s.a_empty[ks]);
+        product_rows<DP, kBf16>(tdq, tdp, k_addr + ks * L::kTileBytes, j == 0);
+        if (elect_one()) mma_commit(&s.a_empty[ks]);
         if (more) {
-          if (!(ok = bar_wait(&s.b_full[vr.stage], vr.phase, &g_timeouts))) break;
-          product_cols<DP, kBf16>(leader, tdp, ga, v_addr + vr.stage * L::kTileBytes);
-          if (leader) {
+          if (!(ok = bar_wait_warp(&s.b_full[vr.stage], vr.phase, &g_timeouts))) break;
+          product_cols<DP, kBf16>(tdp, ga, v_addr + vr.stage * L::kTileBytes);
+          if (elect_one()) {
             mma_commit(&s.dp_full);
             mma_commit(&s.b_empty[vr.stage]);
           }
         }
       }
-      if (leader) mma_commit(&s.done);
-      bar_wait(&s.done, 0, &g_timeouts);
+      if (elect_one()) mma_commit(&s.done);
+      bar_wait_warp(&s.done, 0, &g_timeouts);
     } else if (warp == 9 && n > 0) {
       if (lane == 0) {
         bar_expect(&s.own_full, 2 * L::kTileBytes);

@@ -140,9 +140,9 @@ __device__ __forceinline__ float lse_of(float top, float sum) {
 
 // S = q k^T of one tile of each.
 template <int DP>
-__device__ __forceinline__ void score(bool leader, uint32_t to, uint32_t q, uint32_t k, uint32_t desc) {
+__device__ __forceinline__ void score(uint32_t to, uint32_t q, uint32_t k, uint32_t desc) {
   const TileDesc qd(q, 16), kd(k, 16);
-  if (leader) {
+  if (elect_one()) {
 #pragma unroll
     for (int c = 0; c < DP / 16; ++c) {
       const uint32_t off = (c / 4) * Layout<DP>::kPanel + (c % 4) * 32;
@@ -152,9 +152,9 @@ __device__ __forceinline__ void score(bool leader, uint32_t to, uint32_t q, uint
 }
 // O += P v.
 template <int DP, bool kBf16>
-__device__ __forceinline__ void output(bool leader, uint32_t to, uint32_t p, uint32_t v, bool first) {
+__device__ __forceinline__ void output(uint32_t to, uint32_t p, uint32_t v, bool first) {
   const TileDesc vd(v, Layout<DP>::kPanel);
-  if (leader) {
+  if (elect_one()) {
 #pragma unroll
     for (int c = 0; c < kTile / 16; ++c)
       mma_ts(to, p + c * 8, vd.at(c * 2048), mma_desc(kBf16, DP, true), !first || c > 0);
@@ -177,7 +177,7 @@ __device__ __forceinline__ void load_kv(uint8_t* dst, const CUtensorMap* map, in
     for (int c = 0; c < DP / 64; ++c) tma_load(dst + c * Layout<DP>::kPanel, map, 64 * c, head, (int)row, bar);
   }
   if (clear) {
-    bar_wait(tail, 0, &g_timeouts);
+    bar_wait_warp(tail, 0, &g_timeouts);
     for (int c = 0; c < DP / 64; ++c)
       for (int b = valid * 8 + lane; b < kTile * 8; b += 32)
         reinterpret_cast<uint4*>(dst + c * Layout<DP>::kPanel)[b] = make_uint4(0, 0, 0, 0);
@@ -213,9 +213,7 @@ __global__ void __launch_bounds__(256, 2)
   const int h = blockIdx.x % a.heads, m = h / (a.heads / a.kv_heads);
 
   if (warp == 0) {
-    Tile t = find_tile<false>(a, kTile, blockIdx.x / a.heads);
-    // causal: the last tiles, which see the most keys, start first (a block without a tile has index 0 and no rows)
-    t.index = t.part < 0 ? 0 : t.tiles - 1 - t.index;
+    const Tile t = find_tile<false>(a, kTile, blockIdx.x / a.heads);
     if (lane == 0) s.tile = t;
   } else if (warp == 1 && lane == 0) {
     bar_init(&s.q_full, 1);
@@ -255,7 +253,7 @@ __global__ void __launch_bounds__(256, 2)
     float top = -INFINITY, sum = 0.f;
     bool ok = true;
     for (int j = 0; j < n; ++j) {
-      if (!(ok = bar_wait(&s.s_full, j & 1, &g_timeouts))) break;
+      if (!(ok = bar_wait_warp(&s.s_full, j & 1, &g_timeouts))) break;
       tc_fence_after();
       uint32_t x[kTile];
 #pragma unroll
@@ -267,7 +265,7 @@ __global__ void __launch_bounds__(256, 2)
       if ((j + 1) * kTile > warp_sees) hide(x, sees - j * kTile);
       const float keep = move_top(top, row_max(x) * c);
       if (j > 0) {  // the last product has read P and left O
-        if (!(ok = bar_wait(&s.pv_done, (j - 1) & 1, &g_timeouts))) break;
+        if (!(ok = bar_wait_warp(&s.pv_done, (j - 1) & 1, &g_timeouts))) break;
         tc_fence_after();
         if (__any_sync(0xffffffffu, keep != 1.f)) scale_o<DP>(to + lanes, keep);
       }
@@ -277,7 +275,7 @@ __global__ void __launch_bounds__(256, 2)
       bar_arrive_warp(&s.p_ready);
     }
     if (ok && n > 0) {
-      ok = bar_wait(&s.pv_done, (n - 1) & 1, &g_timeouts);
+      ok = bar_wait_warp(&s.pv_done, (n - 1) & 1, &g_timeouts);
       tc_fence_after();
     }
     if (ok) {
@@ -289,14 +287,13 @@ __global__ void __launch_bounds__(256, 2)
     regs_shrink<56>();
     if (warp == 4 && n > 0) {
       const uint32_t ds = mma_desc(kBf16, kTile, false) | (a.scale < 0.f ? kNegateA : 0u);
-      const bool leader = elect_one();
       const uint32_t q_addr = smem_u32(sq), kv_addr = smem_u32(skv);
       // tiles come as k0 k1 v0 k2 v1 ..: the scores run one tile ahead
       int stage = 0;
       uint32_t phase = 0;
       auto next = [&](int& at) {
         at = stage;
-        if (!bar_wait(&s.kv_full[stage], phase, &g_timeouts)) return false;
+        if (!bar_wait_warp(&s.kv_full[stage], phase, &g_timeouts)) return false;
         if (++stage == kOneStages) {
           stage = 0;
           phase ^= 1;
@@ -304,35 +301,35 @@ __global__ void __launch_bounds__(256, 2)
         return true;
       };
       int at = 0;
-      bool ok = bar_wait(&s.q_full, 0, &g_timeouts) && next(at);
+      bool ok = bar_wait_warp(&s.q_full, 0, &g_timeouts) && next(at);
       if (ok) {
         tc_fence_after();
-        score<DP>(leader, ts, q_addr, kv_addr, ds);
-        if (leader) {
+        score<DP>(ts, q_addr, kv_addr, ds);
+        if (elect_one()) {
           mma_commit(&s.s_full);
           mma_commit(&s.kv_empty[0]);
         }
       }
       for (int j = 0; j < n && ok; ++j) {
         if (j + 1 < n) {
-          if (!(ok = next(at) && bar_wait(&s.s_read, j & 1, &g_timeouts))) break;
+          if (!(ok = next(at) && bar_wait_warp(&s.s_read, j & 1, &g_timeouts))) break;
           tc_fence_after();
-          score<DP>(leader, ts, q_addr, kv_addr + at * L::kTileBytes, ds);
-          if (leader) {
+          score<DP>(ts, q_addr, kv_addr + at * L::kTileBytes, ds);
+          if (elect_one()) {
             mma_commit(&s.s_full);
             mma_commit(&s.kv_empty[at]);
           }
         }
-        if (!(ok = next(at) && bar_wait(&s.p_ready, j & 1, &g_timeouts))) break;
+        if (!(ok = next(at) && bar_wait_warp(&s.p_ready, j & 1, &g_timeouts))) break;
         tc_fence_after();
-        output<DP, kBf16>(leader, to, tp, kv_addr + at * L::kTileBytes, j == 0);
-        if (leader) {
+        output<DP, kBf16>(to, tp, kv_addr + at * L::kTileBytes, j == 0);
+        if (elect_one()) {
           mma_commit(&s.pv_done);
           mma_commit(&s.kv_empty[at]);
         }
       }
-      if (leader) mma_commit(&s.drained);  // nothing leaves before its products are done
-      bar_wait(&s.drained, 0, &g_timeouts);
+      if (elect_one()) mma_commit(&s.drained);  // nothing leaves before its products are done
+      bar_wait_warp(&s.drained, 0, &g_timeouts);
     } else if (warp == 5 && n > 0) {
       if (lane == 0) {
         bar_expect(&s.q_full, L::kTileBytes);
@@ -394,8 +391,7 @@ __global__ void __launch_bounds__(512, 1)
 
   if (warp == 0) {
     Tile t = find_tile<false>(a, 2 * kTile, blockIdx.x / a.heads);
-    // causal: the last tiles, which see the most keys, start first (a block without a tile has index 0 and no rows)
-    t.index = t.part < 0 ? 0 : 2 * (t.tiles - 1 - t.index);
+    t.index *= 2;
     if (lane == 0) s.tile = t;
   } else if (warp == 1 && lane == 0) {
     bar_init(&s.q_full, 1);
@@ -441,7 +437,7 @@ __global__ void __launch_bounds__(512, 1)
     const float c = exponent_factor(a.scale);
     float top = -INFINITY, sum = 0.f;
     for (int j = 0; j < steps; ++j) {
-      if (!bar_wait(&s.s_full[t], j & 1, &g_timeouts)) break;
+      if (!bar_wait_warp(&s.s_full[t], j & 1, &g_timeouts)) break;
       tc_fence_after();
       uint32_t x[kTile];
 #pragma unroll
@@ -468,7 +464,7 @@ __global__ void __launch_bounds__(512, 1)
     for (int j = 0; j < n && ok; ++j) {
       for (int t = 0; t < 2; ++t) {
         if (j >= (t ? n1 : n0)) continue;
-        if (!(ok = bar_wait(&s.grown[t], j & 1, &g_timeouts))) break;
+        if (!(ok = bar_wait_warp(&s.grown[t], j & 1, &g_timeouts))) break;
         const float keep = s.scale[t][row];
         // O holds the keys before: the softmax has had this step's scores, which were issued behind their product
         if (j > 0 && __any_sync(0xffffffffu, keep != 1.f)) {
@@ -481,8 +477,8 @@ __global__ void __launch_bounds__(512, 1)
     }
     for (int t = 0; t < 2 && ok; ++t) {
       const int steps = t ? n1 : n0, i = (tile0 + t) * kTile + row;
-      if (!(ok = bar_wait(&s.sums[t], 0, &g_timeouts) &&
-                 (steps == 0 || bar_wait(&s.o_full[t], 0, &g_timeouts))))
+      if (!(ok = bar_wait_warp(&s.sums[t], 0, &g_timeouts) &&
+                 (steps == 0 || bar_wait_warp(&s.o_full[t], 0, &g_timeouts))))
         break;
       tc_fence_after();
       T* out = static_cast<T*>(a.out) + ((place.q0 + i) * a.heads + h) * a.dim;
@@ -492,13 +488,12 @@ __global__ void __launch_bounds__(512, 1)
     regs_shrink<64>();
     if (warp == 12 && n > 0) {
       const uint32_t ds = mma_desc(kBf16, kTile, false) | (a.scale < 0.f ? kNegateA : 0u);
-      const bool leader = elect_one();
       const uint32_t kv_addr = smem_u32(skv), q_addr = smem_u32(sq);
       int stage = 0;
       uint32_t phase = 0;
       auto next = [&](int& at) {
         at = stage;
-        if (!bar_wait(&s.kv_full[stage], phase, &g_timeouts)) return false;
+        if (!bar_wait_warp(&s.kv_full[stage], phase, &g_timeouts)) return false;
         if (++stage == kTwoStages) {
           stage = 0;
           phase ^= 1;
@@ -506,16 +501,16 @@ __global__ void __launch_bounds__(512, 1)
         return true;
       };
       auto scores = [&](int t, int at) {
-        score<DP>(leader, tmem + t * kTile, q_addr + t * L::kTileBytes, kv_addr + at * L::kTileBytes, ds);
-        if (leader) mma_commit(&s.s_full[t]);
+        score<DP>(tmem + t * kTile, q_addr + t * L::kTileBytes, kv_addr + at * L::kTileBytes, ds);
+        if (elect_one()) mma_commit(&s.s_full[t]);
       };
       int vs = 0, ks = 0;
-      bool ok = bar_wait(&s.q_full, 0, &g_timeouts) && next(ks);
+      bool ok = bar_wait_warp(&s.q_full, 0, &g_timeouts) && next(ks);
       if (ok) {
         tc_fence_after();
         if (n0 > 0) scores(0, 0);
         if (n1 > 0) scores(1, 0);
-        if (leader) mma_commit(&s.kv_empty[0]);
+        if (elect_one()) mma_commit(&s.kv_empty[0]);
       }
       for (int j = 0; j < n && ok; ++j) {
         const bool more = j + 1 < n;
@@ -524,20 +519,20 @@ __global__ void __launch_bounds__(512, 1)
         for (int t = 0; t < 2; ++t) {
           const int steps = t ? n1 : n0;
           if (j >= steps) continue;
-          if (!(ok = bar_wait(&s.p_ready[t], j & 1, &g_timeouts))) break;
+          if (!(ok = bar_wait_warp(&s.p_ready[t], j & 1, &g_timeouts))) break;
           tc_fence_after();
-          output<DP, kBf16>(leader, to + t * DP, tmem + t * kTile, kv_addr + vs * L::kTileBytes, j == 0);
+          output<DP, kBf16>(to + t * DP, tmem + t * kTile, kv_addr + vs * L::kTileBytes, j == 0);
           if (j + 1 < steps) scores(t, ks);
-          else if (leader) mma_commit(&s.o_full[t]);
+          else if (elect_one()) mma_commit(&s.o_full[t]);
         }
         if (!ok) break;
-        if (leader) {
+        if (elect_one()) {
           mma_commit(&s.kv_empty[vs]);
           if (more) mma_commit(&s.kv_empty[ks]);
         }
       }
-      if (leader) mma_commit(&s.drained);  // nothing leaves before its products are done
-      bar_wait(&s.drained, 0, &g_timeouts);
+      if (elect_one()) mma_commit(&s.drained);  // nothing leaves before its products are done
+      bar_wait_warp(&s.drained, 0, &g_timeouts);
     } else if (warp == 13 && n > 0) {
       const int64_t q0 = place.q0 + (int64_t)tile0 * kTile;
       if (lane == 0) {

@@ -57,6 +57,14 @@ __device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, unsigne
   return false;
 }
 
+// The same by a whole warp, with one answer.  It is entered together: lanes that
+// ran ahead of a leader into the wait could spin there while the leader has not
+// yet issued what they wait for.
+__device__ __forceinline__ bool bar_wait_warp(uint64_t* bar, uint32_t parity, unsigned long long* timeouts) {
+  __syncwarp();
+  return __all_sync(0xffffffffu, bar_wait(bar, parity, timeouts));
+}
+
 __device__ __forceinline__ void fence_bar_init() { asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
 // Makes this thread's shared-memory writes visible to TMA and the tensor cores.
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
@@ -103,12 +111,17 @@ struct TileDesc {
   }
 };
 
-// True in one lane of a converged warp.  The warp that issues products runs
-// its loop with all lanes, so that addresses and descriptors stay in uniform
-// registers, and only the products themselves under this.
+// True in one lane of the warp, the same one every time.  The warp that issues
+// products runs its loop with all lanes, so that addresses and descriptors stay in
+// uniform registers, and only the products and their completions under this (with
+// a plain test for lane 0 a product took 90 cycles to issue instead of its 64).
+// It is asked for anew at each place and with the warp together: kept in a
+// variable over the loop it was found to name another lane where the warp had
+// parted, and completions were signalled twice.
 __device__ __forceinline__ bool elect_one() {
   uint32_t one;
-  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(one));
+  __syncwarp();
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(one) : : "memory");
   return one != 0;
 }
 

@@ -9,6 +9,10 @@ Drop-in replacements for the reference's operator modules:
   dynamic_voxelize, dynamic_point_to_voxel_forward,
   dynamic_point_to_voxel_backward}``                      <- ``ops.voxel.voxel_layer.*``
 
+Beside them, without a reference counterpart: attention over active sites
+(``ops.spconv``: ``packed_attention``, ``qk_norm_rotary``,
+``residual_dropout``, ``SparseSelfAttention``).
+
 All kernels live in ``libbfb_b200.so`` (C ABI, include/bfb_b200.h); torch
 custom ops in ``_bfb_torch.so`` wrap it.  There is no CPU or Triton path.
 """

@@ -92,8 +92,9 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, in
     ``inv_freq`` (fp32 or fp64), is half the rotated width R <= dim.  A pair is
     (i, i + R / 2), with R a multiple of 16, or with ``interleaved``
     (2 i, 2 i + 1); values past R are not turned.  ``positions`` [tokens, axes]
-    is int32, int64 or fp32, of any strides; angles are exact to fp32 at any
-    position.  Differentiable in ``q``, ``k`` and the weights.
+    is int32, int64 or fp32, of any strides; far positions lose no accuracy
+    (sine and cosine are good to fp32 for fp32 tensors, to 2 ** -20 for the
+    others).  Differentiable in ``q``, ``k`` and the weights.
     """
     _require_cuda(q, k, positions, inv_freq)
     if q_weight is not None and q_weight.dtype != torch.float32:

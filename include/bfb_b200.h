@@ -532,8 +532,10 @@ int bfb_attention_timeouts(uint64_t* count, int reset);
  * rotated / 2: the first sections[0] pairs follow axis 0, and so on).
  * rotated: a multiple of 16 (of 2 when interleaved).  Positions: element
  * strides position_row and position_axis, position_type 0 = int32, 1 = int64,
- * 2 = f32; inv_freq f32 or (inv_freq_f64) f64.  Angles are reduced in f64, so
- * far positions are exact to f32.
+ * 2 = f32; inv_freq f32 or (inv_freq_f64) f64.  Angles are reduced to a
+ * fraction of a turn in about 48 bits (f64 for the farthest), so far positions
+ * lose nothing; sine and cosine of it are good to f32 for f32 tensors and to
+ * 2^-20 for f16 and bf16.  heads and kv_heads up to 4096.
  *
  * Backward: gradients of q and k (contiguous), and of the weights where given
  * (f32 [dim], summed over tokens and heads in a fixed order). */

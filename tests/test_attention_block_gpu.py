@@ -362,6 +362,65 @@ def test_many_streams(cuda, seqs, heads, kv):
     both(F16, heads, kv, 128, [1] * seqs, lens_k, causal=False, seed=seqs + 1)
 
 
+@pytest.mark.parametrize('heads,kv', [(6, 2), (4, 1)])
+@pytest.mark.parametrize('dim', [64, 128])
+def test_many_short_sequences_share_heads(cuda, heads, kv, dim):
+    """More sequences than one warp looks at in a step, some empty, some of more than one tile, forward and backward."""
+    rng = np.random.default_rng(dim + heads)
+    lens = [int(n) for n in rng.integers(0, 150, 70)]
+    both(BF16, heads, kv, dim, lens, causal=True, spare=5, seed=dim)
+    both(F16, heads, kv, dim, lens, [int(n) for n in rng.integers(0, 150, 70)], causal=True, seed=heads)
+
+
+@pytest.mark.parametrize('queries', [1, 150])
+def test_keys_past_two_to_the_31(cuda, queries):
+    """The last sequence's keys and their gradients lie past 2 ** 31 elements (and 2 ** 32 bytes)."""
+    heads, kv, dim, far, n = 8, 8, 128, 2_150_000, 300
+    if torch.cuda.mem_get_info()[0] < 40 * 2 ** 30:
+        pytest.skip('needs 40 GB')
+    q, ks, vs, g, _ = make(BF16, heads, kv, dim, [queries], [n], seed=queries)
+    k, v = (torch.zeros((far + n, kv, dim), dtype=BF16, device='cuda') for _ in range(2))
+    k[far:], v[far:] = ks, vs
+    assert k.numel() > 2 ** 31
+    for t in (q, k, v):
+        t.requires_grad_(True)
+    out, lse = packed_attention(q, k, v, offsets([0, queries]), offsets([far, n]), causal=True, return_lse=True)
+    dq, dk, dv = torch.autograd.grad(out, (q, k, v), g)
+    value, tol = oracle.attention(q.detach(), ks, vs, [queries], [n], True, dim ** -0.5, dout=g)
+    for name, x in (('out', out), ('lse', lse), ('dq', dq), ('dk', dk[far:]), ('dv', dv[far:])):
+        oracle.check(x.detach(), value[name], tol[name], name)
+    assert not dk[:far].any() and not dv[:far].any()
+
+
+def test_two_streams_at_once(cuda):
+    """Calls of each kind in flight on two streams give what they give alone."""
+    lens, n = [900, 120, 33], 24
+    train = make(BF16, 8, 2, 128, lens, lens, seed=1)[:4]
+    decode = make(F16, 8, 2, 64, [1] * n, [600] * n, seed=2)[:3]
+    cu, cu_q, cu_k = offsets(lens), offsets([1] * n), offsets([600] * n)
+    x = torch.randn((1000, 64), device='cuda')
+    seed = torch.tensor([3, 4], device='cuda')
+
+    def run():
+        a, b, c = (t.detach().requires_grad_(True) for t in train[:3])
+        out = packed_attention(a, b, c, cu, causal=True)
+        return (out.detach(), *torch.autograd.grad(out, (a, b, c), train[3]),
+                packed_attention(*decode, cu_q, cu_k), residual_dropout(x, x, 0.3, seed))
+
+    want = run()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    found = []
+    for _ in range(4):
+        for stream in streams:
+            with torch.cuda.stream(stream):
+                found.append(run())
+    torch.cuda.synchronize()
+    for got in found:
+        for a, b in zip(got, want):
+            assert torch.equal(a, b)
+
+
 def test_second_derivative_is_refused(cuda):
     q, k, v, g, _ = make(F16, 2, 2, 64, [20], [20])
     q.requires_grad_(True)
@@ -458,6 +517,18 @@ def test_rotary_dims_and_sections(cuda, dtype, dim, sections, inter):
 @pytest.mark.parametrize('norm', [False, True])
 def test_rotary_tokens(cuda, tokens, heads, kv, norm):
     rotary_case(BF16, tokens, heads, kv, 64, (8, 12, 12), norm, torch.int64, False, 300, seed=tokens)
+
+
+@pytest.mark.parametrize('dtype,dim,sections,inter', [(BF16, 128, (16, 24, 24), False), (F32, 256, (128,), False),
+                                                      (F16, 24, (5, 7), False), (F16, 24, (5, 7), True)])
+@pytest.mark.parametrize('heads,kv', [(48, 48), (64, 1), (1, 33)])
+def test_rotary_many_heads(cuda, dtype, dim, sections, inter, heads, kv):
+    """More heads than a block has lanes for."""
+    if sum(sections) % 8 and not inter:
+        with pytest.raises(ValueError, match='a multiple of 8, got 12'):
+            rotary_case(dtype, 37, heads, kv, dim, sections, True, torch.int32, inter, 500, seed=heads)
+        return
+    rotary_case(dtype, 37, heads, kv, dim, sections, True, torch.int32, inter, 500, seed=heads)
 
 
 @pytest.mark.parametrize('positions', [torch.int32, torch.int64, torch.float32])

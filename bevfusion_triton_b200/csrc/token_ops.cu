@@ -3,8 +3,12 @@
 // (bfb_qk_norm_rotary, forward and backward) and dropout onto the residual
 // stream from a counter-based generator (bfb_residual_dropout).
 //
-// Both are bound by HBM: every value is read once, worked on in fp32
-// registers, rounded once and written once.
+// Every value is read once, worked on in fp32 registers, rounded once and
+// written once, so HBM is the floor; the instructions are close behind it.
+// Measured: rotary, 24 k tokens of 16 + 4 heads of 128, bf16: forward 58 us,
+// backward 90 us (HBM 41 and 46 % busy, issue 52 and 44 %, 30 and 23 % of the
+// warps fit).  Dropout, 90 k x 512, bf16: with the residual 50 us (HBM 60 %,
+// issue 56 %), its gradient 45 us (37 and 60 %: the generator's ten rounds).
 #include <algorithm>
 #include <cmath>
 #include <type_traits>

@@ -61,7 +61,10 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     sees no key and a row that no sequence holds get 0 (and -inf), and pass
     no gradient.  Rows of ``k`` and ``v`` outside every sequence and past
     ``kv_lengths`` may hold anything; a non-finite ``v`` inside a sequence may
-    reach all queries of that sequence.  Gradients are deterministic.
+    reach all queries of that sequence.  Gradients are deterministic; the
+    probabilities and their gradients are rounded to the inputs' type inside,
+    which in bf16 leaves dq and dk a relative error near 0.0025 (0.0017 with
+    fp32 inside).
     """
     _require_cuda(q, k, v, cu_seqlens_q)
     if scale is None:

@@ -15,11 +15,14 @@
 // dS carries the scale before it is rounded: in fp16 it then overflows only
 // where the gradient itself is near to.
 //
-// delta comes from the rounded o, an error of 2^-9 (bf16) of |dO| |o| that all
-// of a row's dS share.  Over many keys it is lost among them; over few keys,
-// where P is near 1 and dS near 0, it would be most of the result.  So where a
-// sequence's keys fit one tile the dQ kernel sums delta = rowsum(P dP) - dlse
-// in fp32 itself, and leaves it for the dK and dV kernel, which runs second.
+// delta is needed before the walk over the keys that could sum it.  Its first
+// value comes from the rounded o, off by up to 2^-9 (bf16) of |dO| |o|, which
+// all of a row's dS share: where the softmax is peaked (P near 1, dS near 0; the
+// first rows of a causal prompt in any case) that would be most of dQ and dK.
+// So the dQ kernel sums e = rowsum(P (dP - delta)) - dlse's share in fp32 on its
+// walk, which is what delta lacks, keeps P K beside dS K, and subtracts e P K from
+// dQ at the end; delta + e is left for the dK and dV kernel, which runs second.
+// That costs the dQ kernel a fourth product.
 //
 // Measured, one sequence of 8192 tokens, full.  8/2 heads of 128, bf16: dQ 374 us
 // (tensor pipe 55 % busy, special functions 43 %), dK and dV 460 us (61 and 36
@@ -41,6 +44,10 @@ __device__ unsigned long long g_timeouts = 0ull;
 constexpr int kThreads = 384;  // warps 0-7 work on the scores, 8 issues products, 9 loads
 constexpr int kHalf = kTile / 2;
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr uint32_t kNone = 0xffffffffu;  // no place in tensor memory
+
+// The eight warps that work on the scores meet; all of them come here.
+__device__ __forceinline__ void warpgroups_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
 template <int DP>
 struct Layout {
@@ -59,11 +66,11 @@ constexpr int kFirst = 3, kSecond = 2;
 
 struct Shared {
   uint64_t own_full, a_full[kFirst], a_empty[kFirst], b_full[kSecond], b_empty[kSecond];
-  uint64_t s_full, dp_full, p_half, p_ready, ds_ready, halves, done, tail;
+  uint64_t s_full, dp_full, p_half, p_ready, ds_ready, done, tail;
   uint32_t tmem;
   Tile tile;
   alignas(16) float lse2[kFirst][kTile];  // read four at a time
-  alignas(16) float delta[kSecond][kTile];  // dQ: delta's first half row from each warpgroup
+  alignas(16) float delta[kSecond][kTile];  // dQ: what delta lacks, a half row from each warpgroup
 };
 
 template <int DP>
@@ -140,23 +147,32 @@ struct Ring {
 };
 
 // `cols` fp32 columns of a 128-row sum from tensor memory, as 16-bit values
-// [col0, col0 + cols) of a row of [rows, heads, dim].
+// [col0, col0 + cols) of a row of [rows, heads, dim]; less e times those at
+// `less`, where that is given.
 template <class T>
-__device__ __forceinline__ void write_row(uint32_t from, T* out, int col0, int cols, int dim, bool live, bool zero) {
+__device__ __forceinline__ void write_row(uint32_t from, T* out, int col0, int cols, int dim, bool live, bool zero,
+                                          uint32_t less = kNone, float e = 0.f) {
   for (int b = 0; b < cols; b += 32) {
     uint32_t o[32];
     tmem_ld32(from + b, o);
     tmem_ld_wait32(o);
+    if (less != kNone) {
+      uint32_t p[32];
+      tmem_ld32(less + b, p);
+      tmem_ld_wait32(p);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int col = col0 + b + 8 * e;
+      for (int f = 0; f < 32; ++f) o[f] = __float_as_uint(fmaf(-e, __uint_as_float(p[f]), __uint_as_float(o[f])));
+    }
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int col = col0 + b + 8 * g;
       if (!live || col >= dim) continue;
       uint4 w = make_uint4(0, 0, 0, 0);
       uint32_t* ww = reinterpret_cast<uint32_t*>(&w);
       if (!zero) {
 #pragma unroll
         for (int f = 0; f < 4; ++f)
-          ww[f] = pack2<T>(__uint_as_float(o[8 * e + 2 * f]), __uint_as_float(o[8 * e + 2 * f + 1]));
+          ww[f] = pack2<T>(__uint_as_float(o[8 * g + 2 * f]), __uint_as_float(o[8 * g + 2 * f + 1]));
       }
       *reinterpret_cast<uint4*>(out + col) = w;
     }
@@ -185,7 +201,6 @@ __device__ __forceinline__ bool setup(Shared& s, const Args& a, int64_t item) {
       bar_init(&s.p_half, 8);
       bar_init(&s.p_ready, 8);  // one arrival of each warp
       bar_init(&s.ds_ready, 8);
-      bar_init(&s.halves, 8);
       bar_init(&s.done, 1);
       bar_init(&s.tail, 1);
       fence_bar_init();
@@ -466,9 +481,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // ------------------------------------------------------------------------- dQ
-// S = Q K^T, dP = dO V^T, dQ += dS K: a thread owns one query row.  P only
-// lives in registers, so S's columns are free for the next one as soon as
-// they have been read.
+// S = Q K^T, dP = dO V^T, dQ += dS K, and P K beside it: a thread owns one query
+// row.  The order of the steps is that of dK and dV: P K takes dV's place.
 template <class T, int DP>
 __global__ void __launch_bounds__(kThreads, 1)
     dq_kernel(const __grid_constant__ Args a, const __grid_constant__ CUtensorMap q_map,
@@ -483,7 +497,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int h = blockIdx.x % a.heads, m = h / (a.heads / a.kv_heads);
   if (!setup<false>(s, a, blockIdx.x / a.heads)) return;
   const uint32_t tmem = tmem_start(s, warp);
-  const uint32_t ts = tmem, tdp = tmem + kTile, tdq = tmem + 2 * kTile;
+  const uint32_t ts = tmem, tdp = tmem + kTile, tdq = tmem + 2 * kTile, tpk = tdq + DP;
   const Tile place = s.tile;
   const int lq = place.lq, lk = place.lk, i0 = place.index * kTile, shift = lk - lq;
   auto seen = [&](int i) { return a.causal ? max(0, min(lk, i + shift + 1)) : lk; };
@@ -496,8 +510,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const float2 c2 = make_float2(a.scale * kLog2e, a.scale * kLog2e), scale2 = make_float2(a.scale, a.scale);
     const int64_t at = (int64_t)h * a.total_q + place.q0 + i;
     const float lse2 = i < lq ? a.lse2[at] : INFINITY;
-    const bool exact = lk <= kTile;  // one tile of keys: delta is summed here
-    float delta = i < lq && !exact ? a.delta[at] : 0.f;
+    const float delta = i < lq ? a.delta[at] : 0.f;
+    float2 lacks = make_float2(0.f, 0.f);
     const int sees = seen(i), warp_sees = seen(i - lane);
     bool ok = true;
     for (int j = 0; j < n; ++j) {
@@ -508,16 +522,29 @@ __global__ void __launch_bounds__(kThreads, 1)
       tmem_ld32(ts + mine + 32, x + 32);
       tmem_ld_wait32(x);
       tmem_ld_wait32(x + 32);
-      tc_fence_before();
-      bar_arrive_warp(&s.p_ready);  // S is read
       const int limit = sees - j * kTile - wg * kHalf;
       const bool masked = warp_sees < j * kTile + wg * kHalf + kHalf;
       float p[kHalf];
 #pragma unroll
-      for (int e = 0; e < kHalf; e += 2) {
-        const float2 u = fma2(pair_of(x + e), c2, make_float2(-lse2, -lse2));
-        p[e] = exp2_approx(u.x);
-        p[e + 1] = exp2_approx(u.y);
+      for (int b = 0; b < 2; ++b) {
+        uint32_t w[16];
+#pragma unroll
+        for (int e = 32 * b; e < 32 * b + 32; e += 2) {
+          const float2 u = fma2(pair_of(x + e), c2, make_float2(-lse2, -lse2));
+          p[e] = exp2_approx(u.x);
+          p[e + 1] = exp2_approx(u.y);
+          if (masked) {
+            if (e >= limit) p[e] = 0.f;
+            if (e + 1 >= limit) p[e + 1] = 0.f;
+          }
+          w[e / 2 - 16 * b] = pack2<T>(p[e], p[e + 1]);
+        }
+        tmem_st16(ts + mine + 16 * b, w);
+        if (b == 1 || L::kSplit) {
+          tmem_st_wait();
+          tc_fence_before();
+          bar_arrive_warp(b ? &s.p_ready : &s.p_half);
+        }
       }
       if (!(ok = bar_wait_warp(&s.dp_full, j & 1, &g_timeouts))) break;
       tc_fence_after();
@@ -525,18 +552,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       tmem_ld32(tdp + mine + 32, x + 32);
       tmem_ld_wait32(x);
       tmem_ld_wait32(x + 32);
-      if (exact) {
-        float part = 0.f;
-#pragma unroll
-        for (int e = 0; e < kHalf; ++e) part += e < limit ? p[e] * __uint_as_float(x[e]) : 0.f;
-        s.delta[wg][row] = part;
-        bar_arrive_warp(&s.halves);  // the two warpgroups; once, as there is one tile
-        if (!(ok = bar_wait_warp(&s.halves, 0, &g_timeouts))) break;
-        if (i < lq) {
-          delta = a.scale * (s.delta[0][row] + s.delta[1][row] - (a.dlse ? a.dlse[at] : 0.f));
-          if (wg == 0) a.delta[at] = delta;
-        }
-      }
 #pragma unroll
       for (int b = 0; b < 2; ++b) {
         uint32_t w[16];
@@ -549,6 +564,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (col >= limit) u.x = 0.f;
             if (col + 1 >= limit) u.y = 0.f;
           }
+          lacks = add2(lacks, u);
           w[e] = pack2<T>(u.x, u.y);
         }
         tmem_st16(tdp + mine + 16 * b, w);
@@ -557,10 +573,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_before();
       bar_arrive_warp(&s.ds_ready);
     }
+    s.delta[wg][row] = lacks.x + lacks.y;
+    warpgroups_sync();
+    // of a row that sees no key nothing is read
+    const bool live = i < lq && lse2 != INFINITY;
+    const float e = live ? s.delta[0][row] + s.delta[1][row] - (a.dlse ? a.scale * a.dlse[at] : 0.f) : 0.f;
+    if (ok && live && wg == 0) a.delta[at] = delta + e;
     if (ok && (n == 0 || bar_wait_warp(&s.done, 0, &g_timeouts))) {
       tc_fence_after();
       T* out = static_cast<T*>(a.dq) + ((place.q0 + i) * a.heads + h) * a.dim;
-      write_row<T>(tdq + lanes + wg * (DP / 2), out, wg * (DP / 2), DP / 2, a.dim, i < lq, n == 0);
+      const int col0 = wg * (DP / 2);
+      write_row<T>(tdq + lanes + col0, out, col0, DP / 2, a.dim, i < lq, n == 0, tpk + lanes + col0, e);
     }
   } else {
     regs_shrink<88>();
@@ -583,10 +606,21 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int j = 0; j < n && ok; ++j) {
         const bool more = j + 1 < n;
         const int ks = kr.stage;
+        const uint32_t k_now = k_addr + ks * L::kTileBytes;
         kr.step();
         vr.step();
-        if (!(ok = bar_wait_warp(&s.p_ready, j & 1, &g_timeouts))) break;
-        tc_fence_after();
+        if (L::kSplit) {
+          if (!(ok = bar_wait_warp(&s.p_half, j & 1, &g_timeouts))) break;
+          tc_fence_after();
+          product_rows_half<DP, kBf16>(tpk, ts, k_now, j == 0, 0);
+          if (!(ok = bar_wait_warp(&s.p_ready, j & 1, &g_timeouts))) break;
+          tc_fence_after();
+          product_rows_half<DP, kBf16>(tpk, ts, k_now, false, 2);
+        } else {
+          if (!(ok = bar_wait_warp(&s.p_ready, j & 1, &g_timeouts))) break;
+          tc_fence_after();
+          product_rows<DP, kBf16>(tpk, ts, k_now, j == 0);
+        }
         if (more) {
           if (!(ok = bar_wait_warp(&s.a_full[kr.stage], kr.phase, &g_timeouts))) break;
           product_cols<DP, kBf16>(ts, qa, k_addr + kr.stage * L::kTileBytes);
@@ -594,7 +628,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (!(ok = bar_wait_warp(&s.ds_ready, j & 1, &g_timeouts))) break;
         tc_fence_after();
-        product_rows<DP, kBf16>(tdq, tdp, k_addr + ks * L::kTileBytes, j == 0);
+        product_rows<DP, kBf16>(tdq, tdp, k_now, j == 0);
         if (elect_one()) mma_commit(&s.a_empty[ks]);
         if (more) {
           if (!(ok = bar_wait_warp(&s.b_full[vr.stage], vr.phase, &g_timeouts))) break;

@@ -81,8 +81,8 @@ extern "C" int bfb_packed_attention_workspace_size(int64_t total_q, int64_t tota
     return BFB_ERR_INVALID_ARG;
   Carver c(nullptr);
   if (backward) {
-    c.take<float>((size_t)(total_q * heads));
-    c.take<float>((size_t)(total_q * heads));
+    for (int i = 0; i < 3; ++i) c.take<float>((size_t)(total_q * heads));
+    c.take<float>((size_t)(total_k * kv_heads));
   } else if (few_rows(total_q, heads, kv_heads, seqs)) {
     c.take<float>(attn::rows_record_floats((int)dim));
   }
@@ -149,6 +149,8 @@ extern "C" int bfb_packed_attention_backward(
   Carver c(workspace_dev);
   a.lse2 = c.take<float>((size_t)(total_q * heads));
   a.delta = c.take<float>((size_t)(total_q * heads));
+  a.norm_g = c.take<float>((size_t)(total_q * heads));
+  a.norm_v = c.take<float>((size_t)(total_k * kv_heads));
   if (total_q == 0 && total_k == 0) return BFB_OK;
   return attn::backward_sm100(a, dtype, as_stream(stream));
 }

@@ -20,7 +20,8 @@ struct Args {
   // backward
   const void* dout;
   const float* dlse;     // may be NULL
-  float *lse2, *delta;   // workspace, [heads, total_q] each
+  float *lse2, *delta, *norm_g;  // workspace, [heads, total_q] each; norms of the rows of dout
+  float* norm_v;                 // workspace, [kv_heads, total_k]; fp16 alone needs the norms
   void *dq, *dk, *dv;
 };
 

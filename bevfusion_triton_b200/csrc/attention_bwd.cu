@@ -12,8 +12,15 @@
 // of what dQ and dK lose: relative errors of 0.0025 in bf16 and 0.0003 in fp16
 // against 64 bits, where fp32 inside has 0.0017 and 0.0002); each 128 x 128 step is
 // worked by two warpgroups, one per 64 columns, with 64 values per thread.
-// dS carries the scale before it is rounded: in fp16 it then overflows only
-// where the gradient itself is near to.
+//
+// fp16 has few numbers below 2^-14, and dS = P (..) is small as soon as the keys
+// are many or the incoming gradient is (a mean over tokens): rounded as it is it
+// loses its bits there, most entries at last.  So each row of dS, a query's in
+// the dQ kernel and a key's in the other, is taken times a power of two that
+// brings its bound |scale| |dO| |v| + |delta| (norms; the largest of what the row
+// meets) to 2^13, and the fp32 sum is divided by it; entries down to 2^-27 of the
+// bound keep all bits.  P is taken times 2^15 in the same way.  Exact in fp32, and
+// bf16, whose range is fp32's, needs none of it.
 //
 // delta is needed before the walk over the keys that could sum it.  Its first
 // value comes from the rounded o, off by up to 2^-9 (bf16) of |dO| |o|, which
@@ -29,6 +36,7 @@
 // %); 8 heads of 64, fp16: 315 us (32 and 50 %) and 424 us (32 and 37 %).  The
 // chain of a step bounds them, with one block to an SM.
 #include <algorithm>
+#include <cfloat>
 
 #include "attention.cuh"
 
@@ -44,6 +52,7 @@ __device__ unsigned long long g_timeouts = 0ull;
 constexpr int kThreads = 384;  // warps 0-7 work on the scores, 8 issues products, 9 loads
 constexpr int kHalf = kTile / 2;
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kUp = 15.f, kDown = 1.f / 32768.f;  // fp16: log2 of P's factor, and its inverse
 constexpr uint32_t kNone = 0xffffffffu;  // no place in tensor memory
 
 // The eight warps that work on the scores meet; all of them come here.
@@ -69,6 +78,7 @@ struct Shared {
   uint64_t s_full, dp_full, p_half, p_ready, ds_ready, done, tail;
   uint32_t tmem;
   Tile tile;
+  float2 most[8];
   alignas(16) float lse2[kFirst][kTile];  // read four at a time
   alignas(16) float delta[kSecond][kTile];  // dQ: what delta lacks, a half row from each warpgroup
 };
@@ -147,11 +157,11 @@ struct Ring {
 };
 
 // `cols` fp32 columns of a 128-row sum from tensor memory, as 16-bit values
-// [col0, col0 + cols) of a row of [rows, heads, dim]; less e times those at
-// `less`, where that is given.
+// [col0, col0 + cols) of a row of [rows, heads, dim], times `by`; less e times
+// those at `less`, where that is given.
 template <class T>
 __device__ __forceinline__ void write_row(uint32_t from, T* out, int col0, int cols, int dim, bool live, bool zero,
-                                          uint32_t less = kNone, float e = 0.f) {
+                                          float by, uint32_t less = kNone, float e = 0.f) {
   for (int b = 0; b < cols; b += 32) {
     uint32_t o[32];
     tmem_ld32(from + b, o);
@@ -172,7 +182,7 @@ __device__ __forceinline__ void write_row(uint32_t from, T* out, int col0, int c
       if (!zero) {
 #pragma unroll
         for (int f = 0; f < 4; ++f)
-          ww[f] = pack2<T>(__uint_as_float(o[8 * g + 2 * f]), __uint_as_float(o[8 * g + 2 * f + 1]));
+          ww[f] = pack2<T>(__uint_as_float(o[8 * g + 2 * f]) * by, __uint_as_float(o[8 * g + 2 * f + 1]) * by);
       }
       *reinterpret_cast<uint4*>(out + col) = w;
     }
@@ -226,22 +236,48 @@ __device__ __forceinline__ void tmem_end(Shared& s, int warp) {
   }
 }
 
+// The largest x and the largest y of all threads of the warps that work on the
+// scores; once in a block.
+__device__ __forceinline__ float2 largest(Shared& s, float x, float y) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+    y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, o));
+  }
+  if ((threadIdx.x & 31) == 0) s.most[threadIdx.x >> 5] = make_float2(x, y);
+  warpgroups_sync();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    x = fmaxf(x, s.most[i].x);
+    y = fmaxf(y, s.most[i].y);
+  }
+  return make_float2(x, y);
+}
+
+// The power of two that brings `bound` into [2^13, 2^14): sums stay below fp16's
+// 65504 with room for roundings.  1 where there is no such bound.
+__device__ __forceinline__ float lift(float bound) {
+  if (!(bound >= FLT_MIN && bound <= FLT_MAX)) return 1.f;
+  const int e = max((int)(__float_as_uint(bound) >> 23) - 127, -100);
+  return __uint_as_float((uint32_t)(127 + 13 - e) << 23);
+}
+
 // One warp's load of a ring's stage: waits for the stage, fetches the rows by
-// TMA with (src, not NULL) one value for each, negated, `past` from row
-// `valid` on, clears the rows from there on (kClear), and signals `full` (two
+// TMA with (src, not NULL) one value for each, negated, `add` added, `past` from
+// row `valid` on, clears the rows from there on (kClear), and signals `full` (two
 // arrivals).  The values are fetched before the wait, all at once: one after
 // another behind it, their latencies were most of a step.
 template <int DP, bool kClear>
 __device__ __forceinline__ bool load_stage(uint8_t* dst, const CUtensorMap* map, int head, int64_t row, int valid,
                                            uint64_t* full, uint64_t* empty, uint32_t parity, uint64_t* tail,
                                            uint32_t& tails, const float* src = nullptr, float* values = nullptr,
-                                           float past = 0.f) {
+                                           float past = 0.f, float add = 0.f) {
   const int lane = threadIdx.x & 31;
   bool ok = true;
   float x[4];
   if (src) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] = lane + 32 * e < valid ? -src[lane + 32 * e] : past;
+    for (int e = 0; e < 4; ++e) x[e] = lane + 32 * e < valid ? add - src[lane + 32 * e] : past;
   }
   if (lane == 0) ok = bar_wait(empty, parity ^ 1, &g_timeouts);
   if (!__shfl_sync(0xffffffffu, ok, 0)) return false;
@@ -314,6 +350,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int wg = warp >> 2, row = threadIdx.x & (kTile - 1), j = j0 + row;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, mine = lanes + wg * kHalf;
     const float2 c2 = make_float2(a.scale * kLog2e, a.scale * kLog2e), scale2 = make_float2(a.scale, a.scale);
+    float f = 1.f;
+    if (!kBf16 && n > 0) {
+      float g = 0.f, d = 0.f;
+      for (int hh = 0; hh < group; ++hh) {  // the rows that see any of these keys
+        const int64_t at = (int64_t)(m * group + hh) * a.total_q + place.q0;
+#pragma unroll 4
+        for (int i = (a.causal ? max(0, j0 - shift) : 0) + (int)threadIdx.x; i < lq; i += 256) {
+          g = fmaxf(g, a.norm_g[at + i]);
+          d = fmaxf(d, fabsf(a.delta[at + i]));
+        }
+      }
+      const float2 most = largest(s, g, d);
+      if (j < lk) f = lift(fabsf(a.scale) * most.x * a.norm_v[(int64_t)m * a.total_k + place.k0 + j] + most.y);
+    }
+    const float2 down2 = make_float2(f * kDown, f * kDown);
     bool ok = true;
     int tile = 0;
     for (int i = 0; i < n; ++i) {
@@ -377,6 +428,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float4 d = delta[at / 4];  // negative
           float2 u = mul2(make_float2(p[at], p[at + 1]), fma2(pair_of(x + at), scale2, make_float2(d.x, d.y)));
           float2 v = mul2(make_float2(p[at + 2], p[at + 3]), fma2(pair_of(x + at + 2), scale2, make_float2(d.z, d.w)));
+          if (!kBf16) {
+            u = mul2(u, down2);
+            v = mul2(v, down2);
+          }
           if (masked) {
             if (at < from) u.x = 0.f;
             if (at + 1 < from) u.y = 0.f;
@@ -395,7 +450,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (ok && (n == 0 || bar_wait_warp(&s.done, 0, &g_timeouts))) {
       tc_fence_after();
       T* out = static_cast<T*>(wg ? a.dk : a.dv) + ((place.k0 + j) * a.kv_heads + m) * a.dim;
-      write_row<T>((wg ? tdk : tdv) + lanes, out, 0, DP, a.dim, j < place.room, n == 0 || j >= lk);
+      write_row<T>((wg ? tdk : tdv) + lanes, out, 0, DP, a.dim, j < place.room, n == 0 || j >= lk,
+                   kBf16 ? 1.f : wg ? 1.f / f : kDown);
     }
   } else {
     regs_shrink<88>();
@@ -463,7 +519,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int64_t at = (int64_t)h * a.total_q + place.q0 + q;
         // rows past the sequence: P = exp2(-inf) = 0
         if (!load_stage<DP, true>(sq + sa * L::kTileBytes, &q_map, h, place.q0 + q, valid, &s.a_full[sa], &s.a_empty[sa],
-                                  (i / kFirst) & 1, &s.tail, tails, a.lse2 + at, s.lse2[sa], -INFINITY))
+                                  (i / kFirst) & 1, &s.tail, tails, a.lse2 + at, s.lse2[sa], -INFINITY, kBf16 ? 0.f : kUp))
           break;
         ++a_loads;
         if (!load_stage<DP, true>(sg + sb * L::kTileBytes, &g_map, h, place.q0 + q, valid, &s.b_full[sb], &s.b_empty[sb],
@@ -507,10 +563,21 @@ __global__ void __launch_bounds__(kThreads, 1)
     regs_grow<208>();
     const int wg = warp >> 2, row = threadIdx.x & (kTile - 1), i = i0 + row;
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, mine = lanes + wg * kHalf;
-    const float2 c2 = make_float2(a.scale * kLog2e, a.scale * kLog2e), scale2 = make_float2(a.scale, a.scale);
+    const float2 c2 = make_float2(a.scale * kLog2e, a.scale * kLog2e);
     const int64_t at = (int64_t)h * a.total_q + place.q0 + i;
     const float lse2 = i < lq ? a.lse2[at] : INFINITY;
     const float delta = i < lq ? a.delta[at] : 0.f;
+    float f = 1.f;
+    if (!kBf16 && n > 0) {
+      float v = 0.f;
+#pragma unroll 4
+      for (int j = threadIdx.x; j < min(lk, n * kTile); j += 256) v = fmaxf(v, a.norm_v[(int64_t)m * a.total_k + place.k0 + j]);
+      v = largest(s, v, 0.f).x;
+      if (i < lq) f = lift(fabsf(a.scale) * a.norm_g[at] * v + fabsf(delta));
+    }
+    const float down = kBf16 ? 1.f : f * kDown, off = (kBf16 ? 0.f : kUp) - lse2;
+    const float2 off2 = make_float2(off, off), scale2 = make_float2(a.scale * down, a.scale * down),
+                 delta2 = make_float2(-delta * down, -delta * down);
     float2 lacks = make_float2(0.f, 0.f);
     const int sees = seen(i), warp_sees = seen(i - lane);
     bool ok = true;
@@ -530,7 +597,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         uint32_t w[16];
 #pragma unroll
         for (int e = 32 * b; e < 32 * b + 32; e += 2) {
-          const float2 u = fma2(pair_of(x + e), c2, make_float2(-lse2, -lse2));
+          const float2 u = fma2(pair_of(x + e), c2, off2);
           p[e] = exp2_approx(u.x);
           p[e + 1] = exp2_approx(u.y);
           if (masked) {
@@ -558,8 +625,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int e = 0; e < 16; ++e) {
           const int col = 32 * b + 2 * e;
-          float2 u = mul2(make_float2(p[col], p[col + 1]),
-                          fma2(pair_of(x + col), scale2, make_float2(-delta, -delta)));
+          float2 u = mul2(make_float2(p[col], p[col + 1]), fma2(pair_of(x + col), scale2, delta2));
           if (masked) {
             if (col >= limit) u.x = 0.f;
             if (col + 1 >= limit) u.y = 0.f;
@@ -577,13 +643,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     warpgroups_sync();
     // of a row that sees no key nothing is read
     const bool live = i < lq && lse2 != INFINITY;
-    const float e = live ? s.delta[0][row] + s.delta[1][row] - (a.dlse ? a.scale * a.dlse[at] : 0.f) : 0.f;
-    if (ok && live && wg == 0) a.delta[at] = delta + e;
+    const float e = live ? s.delta[0][row] + s.delta[1][row] - (a.dlse ? f * a.scale * a.dlse[at] : 0.f) : 0.f;
+    if (ok && live && wg == 0) a.delta[at] = delta + e / f;
     if (ok && (n == 0 || bar_wait_warp(&s.done, 0, &g_timeouts))) {
       tc_fence_after();
       T* out = static_cast<T*>(a.dq) + ((place.q0 + i) * a.heads + h) * a.dim;
       const int col0 = wg * (DP / 2);
-      write_row<T>(tdq + lanes + col0, out, col0, DP / 2, a.dim, i < lq, n == 0, tpk + lanes + col0, e);
+      write_row<T>(tdq + lanes + col0, out, col0, DP / 2, a.dim, i < lq, n == 0, 1.f / f, tpk + lanes + col0,
+                   kBf16 ? e : e * kDown);
     }
   } else {
     regs_shrink<88>();
@@ -667,24 +734,44 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // What both kernels read for each query and head: lse2 = log2(e) lse, +inf
-// where no key is seen (so that P = 0), and delta = scale (rowsum(dO o) - dlse).
+// where no key is seen (so that P = 0), and delta = scale (rowsum(dO o) - dlse);
+// for fp16 the norms of dO's rows, too, and behind these units those of v's.
 // A group of lanes takes a row, 16 bytes each.
 template <class T>
 __global__ void __launch_bounds__(256) rows_kernel(const __grid_constant__ Args a, int lanes) {
-  const int64_t unit = ((int64_t)blockIdx.x * 256 + threadIdx.x) / lanes;  // row * heads + head
+  constexpr bool kNorms = std::is_same<T, __half>::value;
+  int64_t unit = ((int64_t)blockIdx.x * 256 + threadIdx.x) / lanes;  // row * heads + head
   const int lane = threadIdx.x & (lanes - 1);
-  const bool live = unit < a.total_q * a.heads;
-  float d = 0.f;
+  const bool of_v = kNorms && unit >= a.total_q * a.heads;
+  if (of_v) unit -= a.total_q * a.heads;
+  const int heads = of_v ? a.kv_heads : a.heads;
+  const bool live = unit < (of_v ? a.total_k : a.total_q) * heads;
+  const int64_t r = unit / heads, h = unit - r * heads;
+  float d = 0.f, sq = 0.f;
   if (live && lane * 8 < a.dim) {
-    const uint4 x = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.out) + unit * a.dim + lane * 8);
-    const uint4 y = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.dout) + unit * a.dim + lane * 8);
-    const T *u = reinterpret_cast<const T*>(&x), *v = reinterpret_cast<const T*>(&y);
+    const uint4 y = *reinterpret_cast<const uint4*>(
+        (of_v ? static_cast<const T*>(a.v) + r * a.v_row + h * a.v_head : static_cast<const T*>(a.dout) + unit * a.dim) +
+        lane * 8);
+    const T* v = reinterpret_cast<const T*>(&y);
+    if (!of_v) {
+      const uint4 x = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.out) + unit * a.dim + lane * 8);
+      const T* u = reinterpret_cast<const T*>(&x);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) d += to_f32<T>(u[e]) * to_f32<T>(v[e]);
+      for (int e = 0; e < 8; ++e) d += to_f32<T>(u[e]) * to_f32<T>(v[e]);
+    }
+    if (kNorms) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sq += to_f32<T>(v[e]) * to_f32<T>(v[e]);
+    }
   }
-  for (int o = lanes >> 1; o > 0; o >>= 1) d += __shfl_xor_sync(0xffffffffu, d, o);
+  for (int o = lanes >> 1; o > 0; o >>= 1) {
+    d += __shfl_xor_sync(0xffffffffu, d, o);
+    if (kNorms) sq += __shfl_xor_sync(0xffffffffu, sq, o);
+  }
   if (!live || lane > 0) return;
-  const int64_t r = unit / a.heads, at = (unit - r * a.heads) * a.total_q + r;
+  const int64_t at = h * (of_v ? a.total_k : a.total_q) + r;
+  if (kNorms) (of_v ? a.norm_v : a.norm_g)[at] = sqrtf(sq);
+  if (of_v) return;
   const float lse = a.lse[at];
   a.lse2[at] = lse == -INFINITY ? INFINITY : lse * kLog2e;
   a.delta[at] = a.scale * (d - (a.dlse ? a.dlse[at] : 0.f));
@@ -706,7 +793,8 @@ int launch(const Args& a, int dtype, cudaStream_t stream) {
   const int64_t k_blocks = tile_bound(a.total_k, a.seqs, kTile) * a.kv_heads;
   int lanes = 1;
   while (lanes * 8 < a.dim) lanes <<= 1;
-  const int64_t row_blocks = ceil_div(a.total_q * a.heads * lanes, 256);
+  const int64_t norms = dtype == BFB_F16 ? a.total_k * a.kv_heads : 0;
+  const int64_t row_blocks = ceil_div((a.total_q * a.heads + norms) * lanes, 256);
   if (std::max(std::max(q_blocks, k_blocks), row_blocks) > 0x7fffffff) return BFB_ERR_TOO_LARGE;
   if (a.total_q > 0) {
     rows_kernel<T><<<(unsigned)row_blocks, 256, 0, stream>>>(a, lanes);

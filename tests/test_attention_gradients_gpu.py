@@ -1,5 +1,6 @@
 """Gradients of packed_attention where roundings inside the kernels would show:
-rows whose softmax is peaked (dS is then a small difference of large numbers).
+rows whose softmax is peaked (dS is then a small difference of large numbers),
+small incoming gradients in fp16.
 
 The tolerances are counted for a backward that keeps all but the operands of its
 products in fp32.  With u = eps / 2 of the dtype:
@@ -12,7 +13,8 @@ products in fp32.  With u = eps / 2 of the dtype:
 * dP is off by 2^-20 sum |dO| |v|.  delta = sum P dP - dlse is a sum of fp32
   terms around the first estimate, so it is off by (2^-20 + 2 E + chain) of twice
   W = sum P |dO| |v|, and not by the roundings of the output.
-* dS is rounded to the type (u).
+* dS is rounded to the type (u), and only that: a power of two for each row keeps
+  it out of fp16's subnormal numbers, down to 2^-38 of the row's bound.
 * the first estimate takes delta from the rounded output; what that leaves, e, is
   put right by a product with P rounded to the type: 2 u e P |k|.
 """
@@ -22,7 +24,7 @@ import pytest
 import torch
 
 from bevfusion_triton_b200.ops.spconv import packed_attention
-from tests.test_attention_block_gpu import BF16, make, no_wait_gave_up, offsets  # noqa: F401
+from tests.test_attention_block_gpu import BF16, F16, make, no_wait_gave_up, offsets  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -104,7 +106,7 @@ def compare(q, k, v, g, gl, lens_q, lens_k, causal, scale, exact=False):
             f'({float(off.max()):.3g} tolerances; {int((off > 1).sum())} of {off.numel()} are off)')
 
 
-@pytest.mark.parametrize('dtype', [BF16])
+@pytest.mark.parametrize('dtype', [F16, BF16])
 @pytest.mark.parametrize('dim', [64, 128])
 @pytest.mark.parametrize('causal', [False, True])
 @pytest.mark.parametrize('lens', [[129], [700], [2048], [64, 300]])
@@ -115,3 +117,31 @@ def test_peaked_rows(cuda, dtype, dim, causal, lens):
     q, k = ((4 * x).round().clamp(-60, 60) / 4 for x in (4 * q.float(), k.float()))
     compare(q.to(dtype), k.to(dtype), v, g, gl, lens, lens, causal, dim ** -0.5, exact=True)
 
+
+@pytest.mark.parametrize('size', [2.0 ** -7, 2.0 ** -10, 2.0 ** -13])
+@pytest.mark.parametrize('dim', [64, 128])
+@pytest.mark.parametrize('causal', [False, True])
+def test_small_gradients_in_fp16(cuda, size, dim, causal):
+    """A mean over many tokens leaves each a small gradient: dS = P (..) would be subnormal."""
+    lens = [2100, 37]
+    q, k, v, g, _ = make(F16, 2, 1, dim, lens, lens, seed=dim)
+    compare(q, k, v, (g.float() * size).half(), None, lens, lens, causal, dim ** -0.5)
+
+
+@pytest.mark.parametrize('dim', [64, 128])
+def test_many_keys_in_fp16(cuda, dim):
+    """Even attention over 120 k keys: P near 2^-17 is far below fp16's normal numbers; and a gradient of lse."""
+    lens_q, lens_k = [130], [120_000]
+    q, k, v, g, gl = make(F16, 1, 1, dim, lens_q, lens_k, seed=dim)
+    compare(q, k, v, 16 * g, gl, lens_q, lens_k, False, 2.0 ** -10)
+
+
+@pytest.mark.parametrize('causal', [False, True])
+@pytest.mark.parametrize('dim', [40, 128])
+def test_gradients_of_mixed_sizes_in_fp16(cuda, causal, dim):
+    """Rows whose gradients differ by up to 2^14, in a batch with a sequence whose gradients are all zero."""
+    lens = [300, 700, 5]
+    q, k, v, g, gl = make(F16, 4, 2, dim, lens, lens, seed=dim)
+    size = 2.0 ** -(torch.arange(sum(lens), device='cuda') * 37 % 15).float()
+    size[300:] *= torch.cat([torch.zeros(700), torch.ones(5)]).cuda()
+    compare(q, k, v, (g.float() * size[:, None, None]).half(), gl * size, lens, lens, causal, dim ** -0.5)

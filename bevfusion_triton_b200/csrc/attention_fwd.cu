@@ -6,8 +6,11 @@
 //   O += P v         (tcgen05, P from tensor memory)
 // over the keys in tiles of 128; O stays in tensor memory.  Where a row's
 // maximum grows, O and the sum have to be scaled down; here the maximum in use
-// is only moved when it grows by more than 2^8 (P stays below 2^8, far from
-// fp16's range), so the scaling is rare and its result the same.
+// is only moved when it grows by more than 2^8, so the scaling is rare and its
+// result the same (a published idea for this chip, not this file's).  In fp16 m is
+// 7 below the maximum: P stays below 2^15, and the keys of a long tail (2^-14 of
+// the largest and less) out of the subnormal numbers, where each counts for
+// little but all of them together need not.
 //
 // Two kernels, by the width of a head:
 // * up to 64 (one_tile_kernel): a block takes 128 query rows, two blocks fit an
@@ -68,9 +71,12 @@ __device__ __forceinline__ float row_max(const uint32_t (&x)[kTile]) {
   return fmaxf(fmaxf(best[0], best[1]), fmaxf(best[2], best[3]));
 }
 
-// Moves a row's maximum `top` to `now` where it has to, and returns what O and
-// the sum are to be scaled by.
+// Moves m, `top` here, to kBelow under a row's maximum `now` where it has to, and
+// returns what O and the sum are to be scaled by.
+template <class T>
 __device__ __forceinline__ float move_top(float& top, float now) {
+  constexpr float kBelow = std::is_same<T, __half>::value ? 7.f : 0.f;
+  now -= kBelow;
   if (!(now > top + kGrow || top == -INFINITY)) return 1.f;
   const float keep = now == -INFINITY ? 1.f : exp2_approx(top - now);  // 0 at the first keys
   top = now;
@@ -268,7 +274,7 @@ __global__ void __launch_bounds__(256, 2)
       tc_fence_before();
       bar_arrive_warp(&s.s_read);
       if ((j + 1) * kTile > warp_sees) hide(x, sees - j * kTile);
-      const float keep = move_top(top, row_max(x) * c);
+      const float keep = move_top<T>(top, row_max(x) * c);
       if (j > 0) {  // the last product has read P and left O
         if (!(ok = bar_wait_warp(&s.pv_done, (j - 1) & 1, &g_timeouts))) break;
         tc_fence_after();
@@ -450,7 +456,7 @@ __global__ void __launch_bounds__(512, 1)
 #pragma unroll
       for (int b = 0; b < 4; ++b) tmem_ld_wait32(x + 32 * b);
       if ((j + 1) * kTile > warp_sees) hide(x, sees - j * kTile);
-      const float keep = move_top(top, row_max(x) * c);
+      const float keep = move_top<T>(top, row_max(x) * c);
       s.scale[t][row] = keep;
       bar_arrive_warp(&s.grown[t]);
       sum = sum * keep + write_p<T>(x, c, top, ts);

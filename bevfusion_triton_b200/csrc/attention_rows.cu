@@ -133,6 +133,8 @@ __global__ void __launch_bounds__(kThreads, 2)
     rows_kernel(const __grid_constant__ Args a, float* __restrict__ records) {
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float top_s[kWarps][kRows], sum_s[kWarps][kRows];
+  // exponentials are taken from 15 below the maximum in fp16: P up to 2^15, a long tail's keys no subnormal numbers
+  constexpr float kBelow = std::is_same<T, __half>::value ? 15.f : 0.f;
   constexpr int kChunks = DP / 8;  // 16-byte chunks of a row; chunk c of row r sits at c ^ (r % 8)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane & 3, g = lane >> 2;
   const int group = a.heads / a.kv_heads;
@@ -262,7 +264,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         now[e] = fmaxf(now[e], __shfl_xor_sync(0xffffffffu, now[e], 1));
-        now[e] = fmaxf(now[e], __shfl_xor_sync(0xffffffffu, now[e], 2));
+        now[e] = fmaxf(now[e], __shfl_xor_sync(0xffffffffu, now[e], 2)) - kBelow;
       }
       if (__any_sync(0xffffffffu, now[0] > top[0] || now[1] > top[1])) {
 #pragma unroll

@@ -145,3 +145,18 @@ def test_gradients_of_mixed_sizes_in_fp16(cuda, causal, dim):
     size = 2.0 ** -(torch.arange(sum(lens), device='cuda') * 37 % 15).float()
     size[300:] *= torch.cat([torch.zeros(700), torch.ones(5)]).cuda()
     compare(q, k, v, (g.float() * size[:, None, None]).half(), gl * size, lens, lens, causal, dim ** -0.5)
+
+
+@pytest.mark.parametrize('dim', [64, 128])
+@pytest.mark.parametrize('seqs,queries,keys', [(300, 1, 4096), (1, 1, 120_000), (1, 130, 120_000)])
+def test_long_tail_in_fp16(cuda, dim, seqs, queries, keys):
+    """One key 2^26 above all others, which alone have values: their part of the output is keys times 2^-26."""
+    q, k, v, _, _ = make(F16, 2, 1, dim, [queries * seqs], [keys * seqs])
+    q, k, v = torch.zeros_like(q), torch.zeros_like(k), torch.full_like(v, 64)
+    q[..., 0], k[::keys, :, 0], v[::keys] = 1, 26, 0
+    out = packed_attention(q, k, v, offsets([queries] * seqs), offsets([keys] * seqs), scale=math.log(2))
+    tail = (keys - 1) * 2.0 ** -26
+    # P and the result are rounded; the exponent is off by 2^-24 of 26 and the exponential by 2^-22; fp32 sums of
+    # keys / 16 steps
+    tol = 2 * 2.0 ** -11 + 26 * 2.0 ** -23 + 2.0 ** -22 + keys / 16 * 2.0 ** -23
+    assert float((out.double() / (64 * tail / (1 + tail)) - 1).abs().max()) <= tol

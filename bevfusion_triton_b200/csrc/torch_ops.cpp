@@ -1142,6 +1142,13 @@ c10::optional<at::Tensor> or_null(const at::Tensor& t) {
   return t.defined() ? c10::optional<at::Tensor>(t) : c10::nullopt;
 }
 
+// A tangent that came this far would be dropped below autograd, as if it were zero.
+void no_tangents(const char* name, std::initializer_list<const at::Tensor*> ts) {
+  for (const at::Tensor* t : ts)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(/*level=*/0).defined(), name,
+                                " has no forward-mode derivative");
+}
+
 template <class F>
 auto op_handle(const char* name) {
   return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
@@ -1186,6 +1193,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> attention_backward_autograd(
     const at::Tensor& dout, const c10::optional<at::Tensor>& dlse, const at::Tensor& q, const at::Tensor& k,
     const at::Tensor& v, const at::Tensor& out, const at::Tensor& lse, const at::Tensor& cu_q, const at::Tensor& cu_k,
     const c10::optional<at::Tensor>& lengths, bool causal, double scale) {
+  no_tangents("packed_attention", {&dout, &or_none(dlse), &q, &k, &v, &out, &lse});
   if (!wants_grad({&dout, &or_none(dlse), &q, &k, &v, &out, &lse}))
     return call_attention_backward(dout, dlse, q, k, v, out, lse, cu_q, cu_k, lengths, causal, scale);
   auto r = AttentionSecond::apply(dout, dlse, q, k, v, out, lse, cu_q, cu_k, lengths, causal, scale);
@@ -1217,6 +1225,7 @@ std::tuple<at::Tensor, at::Tensor> attention_autograd(const at::Tensor& q, const
                                                       const at::Tensor& cu_q, const at::Tensor& cu_k,
                                                       const c10::optional<at::Tensor>& lengths, bool causal,
                                                       double scale) {
+  no_tangents("packed_attention", {&q, &k, &v});
   if (!wants_grad({&q, &k, &v})) return call_attention(q, k, v, cu_q, cu_k, lengths, causal, scale);
   auto r = AttentionGrad::apply(q, k, v, cu_q, cu_k, lengths, causal, scale);
   return {r[0], r[1]};
@@ -1256,6 +1265,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> rotary_backward_autog
     const at::Tensor& gq, const at::Tensor& gk, const at::Tensor& q, const at::Tensor& k, const at::Tensor& positions,
     const at::Tensor& inv_freq, at::IntArrayRef sections, const c10::optional<at::Tensor>& qw,
     const c10::optional<at::Tensor>& kw, double eps, bool interleaved) {
+  no_tangents("qk_norm_rotary", {&gq, &gk, &q, &k, &positions, &inv_freq, &or_none(qw), &or_none(kw)});
   if (!wants_grad({&gq, &gk, &q, &k, &or_none(qw), &or_none(kw)}))
     return call_rotary_backward(gq, gk, q, k, positions, inv_freq, sections, qw, kw, eps, interleaved);
   auto r = RotarySecond::apply(gq, gk, q, k, positions, inv_freq, sections, qw, kw, eps, interleaved);
@@ -1290,6 +1300,7 @@ std::tuple<at::Tensor, at::Tensor> rotary_autograd(const at::Tensor& q, const at
                                                    at::IntArrayRef sections, const c10::optional<at::Tensor>& qw,
                                                    const c10::optional<at::Tensor>& kw, double eps,
                                                    bool interleaved) {
+  no_tangents("qk_norm_rotary", {&q, &k, &positions, &inv_freq, &or_none(qw), &or_none(kw)});
   if (!wants_grad({&q, &k, &or_none(qw), &or_none(kw)}))
     return call_rotary(q, k, positions, inv_freq, sections, qw, kw, eps, interleaved);
   auto r = RotaryGrad::apply(q, k, positions, inv_freq, sections, qw, kw, eps, interleaved);
@@ -1325,6 +1336,7 @@ struct DropoutGrad : torch::autograd::Function<DropoutGrad> {
 
 at::Tensor dropout_autograd(const at::Tensor& x, const c10::optional<at::Tensor>& residual, double p,
                             const at::Tensor& seed) {
+  no_tangents("residual_dropout", {&x, &or_none(residual)});
   if (!wants_grad({&x, &or_none(residual)})) return call_dropout(x, residual, p, seed);
   return DropoutGrad::apply(x, residual, p, seed);
 }

@@ -134,14 +134,18 @@ class SparseSelfAttention(SparseModule):
     channels // heads, ``qk_norm_rotary`` at the sites' coordinates,
     ``packed_attention``, projection, ``residual_dropout`` onto the input.
 
-    The tensor's rows must be grouped by sample in ascending order, as
-    voxelisation and the sparse convolutions produce them.  Features are fp16 or bf16, or
+    The tensor's rows may come in any order: of several samples they are
+    gathered by sample first (in their order within it) and the result is put
+    back, without a look at the host; ``grouped=True`` promises that they come
+    sample by sample already, in ascending order, as from voxelisation and the
+    strided convolutions, and saves that.  Features are fp16 or bf16, or
     any floating type under ``torch.autocast``; the width of a head is a
-    multiple of 16 up to 128.  ``causal`` lets a site see only the rows up to its own.
+    multiple of 16 up to 128.  ``causal`` lets a site see only the rows of its
+    sample up to its own.
     """
 
     def __init__(self, channels, heads, kv_heads=None, ndim=3, dropout=0.0, causal=False, rotary_base=10000.0,
-                 qk_norm=True, bias=True, eps=1e-6):
+                 qk_norm=True, bias=True, eps=1e-6, grouped=False):
         super().__init__()
         kv_heads = heads if kv_heads is None else kv_heads
         if channels % heads or heads % kv_heads:
@@ -152,7 +156,7 @@ class SparseSelfAttention(SparseModule):
         if not 0.0 <= dropout <= 1.0:
             raise ValueError(f'dropout must be a probability, got {dropout}')
         self.heads, self.kv_heads, self.dim, self.ndim = heads, kv_heads, dim, ndim
-        self.dropout, self.causal, self.eps = dropout, causal, eps
+        self.dropout, self.causal, self.eps, self.grouped = dropout, causal, eps, grouped
         pairs = dim // 2
         # near equal shares of the pairs; the first axes (the coarser ones) get the smaller
         self.sections = [pairs // ndim + (1 if a >= ndim - pairs % ndim else 0) for a in range(ndim)]
@@ -170,12 +174,19 @@ class SparseSelfAttention(SparseModule):
         feats, h, m = input.features, self.heads, self.kv_heads
         if self.inv_freq.device != feats.device:
             self.inv_freq = self.inv_freq.to(feats.device)
-        qkv = self.qkv(self.norm(feats)).unflatten(1, (h + 2 * m, self.dim))
+        rows, sites, back = feats, input.indices, None
+        if input.batch_size > 1 and not self.grouped:
+            order = torch.argsort(sites[:, 0], stable=True)
+            back = torch.empty_like(order).scatter_(0, order, torch.arange(order.numel(), device=order.device))
+            rows, sites = feats.index_select(0, order), sites.index_select(0, order)
+        qkv = self.qkv(self.norm(rows)).unflatten(1, (h + 2 * m, self.dim))
         q, k, v = qkv.split([h, m, m], 1)
-        q, k = qk_norm_rotary(q, k, input.indices[:, 1:], self.inv_freq, self.sections, self.q_weight,
-                              self.k_weight, self.eps)
-        out = packed_attention(q, k, v, sample_offsets(input.indices, input.batch_size), causal=self.causal)
+        q, k = qk_norm_rotary(q, k, sites[:, 1:], self.inv_freq, self.sections, self.q_weight, self.k_weight,
+                              self.eps)
+        out = packed_attention(q, k, v, sample_offsets(sites, input.batch_size), causal=self.causal)
         out = self.proj(out.flatten(1)).to(feats.dtype)
+        if back is not None:
+            out = out.index_select(0, back)
         if self.training and self.dropout > 0:
             seed = torch.randint(-(1 << 63), (1 << 63) - 1, (2,), device=feats.device)
             out = residual_dropout(out, feats, self.dropout, seed)

@@ -1,0 +1,74 @@
+"""SparseSelfAttention on tensors whose rows are not in the order of their samples."""
+import pytest
+import torch
+
+from bevfusion_triton_b200.ops.spconv import SparseConvTensor, SparseSelfAttention, SparseSequential, SubMConv3d
+from tests.test_attention_block_gpu import block64, no_wait_gave_up  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def scan(batch, per, channels, seed):
+    g = torch.Generator().manual_seed(seed)
+    rows = []
+    for b in range(batch):
+        cells = torch.randperm(8 * 30 * 30, generator=g)[:per[b]]
+        rows.append(torch.stack([torch.full_like(cells, b), cells // 900, cells // 30 % 30, cells % 30], 1))
+    indices = torch.cat(rows).int().cuda()
+    return indices, torch.randn(len(indices), channels, generator=g).cuda()
+
+
+@pytest.mark.parametrize('causal', [False, True])
+def test_rows_in_any_order(cuda, causal):
+    """Shuffled rows against the layer's definition in 64 bits, which picks each sample's rows by their index."""
+    torch.manual_seed(1)
+    indices, feats = scan(3, (70, 150, 31), 64, 0)
+    mixed = torch.randperm(len(indices), generator=torch.Generator().manual_seed(5)).cuda()
+    indices, feats = indices[mixed], feats[mixed].requires_grad_(True)
+    layer = SparseSelfAttention(64, 4, 2, causal=causal).cuda()
+    with torch.autocast('cuda', dtype=torch.float16):
+        y = layer(SparseConvTensor(feats, indices, [8, 30, 30], 3))
+    assert y.indices is indices
+    order = torch.argsort(indices[:, 0], stable=True)  # the definition returns the samples one after another
+    want, leaf, params = block64(layer, feats[order], indices[order], 3, None)
+    back = torch.argsort(order)
+    want = want[back]
+    # about ten fp16 roundings in a row, each 2^-11 of values whose sums of products are taken over up to 150 terms
+    close = lambda a, b: (a.double() - b).abs().max() <= 2.0 ** -5 * b.abs().max()  # noqa: E731
+    assert close(y.features.detach(), want.detach())
+    up = torch.randn_like(feats)
+    names = [n for n, _ in layer.named_parameters()]
+    got = torch.autograd.grad(y.features, [feats] + [t for _, t in layer.named_parameters()], up)
+    ref = torch.autograd.grad(want, [leaf] + [params[n] for n in names], up.double())
+    for n, a, b in zip(['features'] + names, got, [ref[0][back], *ref[1:]]):
+        assert close(a, b), n
+
+
+def test_order_of_rows_changes_nothing(cuda):
+    """Whole samples in another order, and samples dealt out in turn: the same bits, each at its row.  (Within a sample
+    the order stays, which the sums follow.)"""
+    torch.manual_seed(2)
+    indices, feats = scan(2, (90, 90), 32, 1)
+    layer = SparseSelfAttention(32, 2, dropout=0.0).cuda().half().eval()
+    feats = feats.half()
+    want = layer(SparseConvTensor(feats, indices, [8, 30, 30], 2)).features
+    n = torch.arange(180, device='cuda')
+    for order in (torch.cat([n[90:], n[:90]]), n.view(2, 90).t().flatten()):
+        got = layer(SparseConvTensor(feats[order], indices[order], [8, 30, 30], 2)).features
+        assert torch.equal(got, want[order])
+    layer.grouped = True  # known to be: the same bits without the gathering
+    assert torch.equal(layer(SparseConvTensor(feats, indices, [8, 30, 30], 2)).features, want)
+
+
+def test_after_a_submanifold_convolution(cuda):
+    """A submanifold convolution hands rows on as they come; a sample's result does not depend on the other's rows."""
+    torch.manual_seed(3)
+    indices, feats = scan(2, (120, 40), 32, 2)
+    stack = SparseSequential(SubMConv3d(32, 32, 3, indice_key='s'), SparseSelfAttention(32, 2)).cuda().half().eval()
+    mixed = torch.randperm(160, generator=torch.Generator().manual_seed(7)).cuda()
+    first = mixed[indices[mixed, 0] == 0]  # sample 0's rows in their mixed order
+    both = stack(SparseConvTensor(feats[mixed].half(), indices[mixed], [8, 30, 30], 2)).features
+    alone = stack(SparseConvTensor(feats[first].half(), indices[first], [8, 30, 30], 1)).features
+    # the convolution's sums over 27 sites and the products of the layer may be blocked otherwise: fp16 roundings
+    diff = (both[indices[mixed, 0] == 0].double() - alone.double()).abs().max()
+    assert diff <= 2.0 ** -6 * alone.double().abs().max()

@@ -91,13 +91,13 @@ static_assert(smem_bytes<128>() <= 227 * 1024, "a block's shared memory");
 // columns: the second half starts 64 columns of tensor memory later.
 __device__ __forceinline__ constexpr uint32_t half_step(int c) { return (c >> 2) * kHalf + (c & 3) * 8; }
 
-// Clears the rows from `valid` on of a tile in shared memory, by one warp.
-// Rows behind a sequence meet zeros of P and dS in the products, but 0 * NaN
-// is not 0.
+// Clears the rows [from, to) of a tile in shared memory, by one warp.  Rows
+// behind a sequence, and queries that see no key, meet zeros of P and dS in the
+// products, but 0 * NaN is not 0.
 template <int DP>
-__device__ __forceinline__ void clear_rows(uint8_t* tile, int valid) {
+__device__ __forceinline__ void clear_rows(uint8_t* tile, int from, int to) {
   for (int c = 0; c < DP / 64; ++c)
-    for (int b = valid * 8 + (threadIdx.x & 31); b < kTile * 8; b += 32)
+    for (int b = from * 8 + (threadIdx.x & 31); b < to * 8; b += 32)
       reinterpret_cast<uint4*>(tile + c * Layout<DP>::kPanel)[b] = make_uint4(0, 0, 0, 0);
 }
 
@@ -264,11 +264,11 @@ __device__ __forceinline__ float lift(float bound) {
 
 // One warp's load of a ring's stage: waits for the stage, fetches the rows by
 // TMA with (src, not NULL) one value for each, negated, `add` added, `past` from
-// row `valid` on, clears the rows from there on (kClear), and signals `full` (two
-// arrivals).  The values are fetched before the wait, all at once: one after
+// row `valid` on, clears the rows from there on and those before `skip` (kClear),
+// and signals `full` (two arrivals).  The values are fetched before the wait, all at once: one after
 // another behind it, their latencies were most of a step.
 template <int DP, bool kClear>
-__device__ __forceinline__ bool load_stage(uint8_t* dst, const CUtensorMap* map, int head, int64_t row, int valid,
+__device__ __forceinline__ bool load_stage(uint8_t* dst, const CUtensorMap* map, int head, int64_t row, int skip, int valid,
                                            uint64_t* full, uint64_t* empty, uint32_t parity, uint64_t* tail,
                                            uint32_t& tails, const float* src = nullptr, float* values = nullptr,
                                            float past = 0.f, float add = 0.f) {
@@ -281,7 +281,7 @@ __device__ __forceinline__ bool load_stage(uint8_t* dst, const CUtensorMap* map,
   }
   if (lane == 0) ok = bar_wait(empty, parity ^ 1, &g_timeouts);
   if (!__shfl_sync(0xffffffffu, ok, 0)) return false;
-  const bool clear = kClear && valid < kTile;
+  const bool clear = kClear && (valid < kTile || skip > 0);
   if (lane == 0) {
     uint64_t* bar = clear ? tail : full;
     bar_expect(bar, Layout<DP>::kTileBytes);
@@ -295,7 +295,8 @@ __device__ __forceinline__ bool load_stage(uint8_t* dst, const CUtensorMap* map,
     ok = bar_wait_warp(tail, tails & 1, &g_timeouts);
     ++tails;
     if (!__all_sync(0xffffffffu, ok)) return false;
-    clear_rows<DP>(dst, valid);
+    clear_rows<DP>(dst, 0, skip);
+    clear_rows<DP>(dst, valid, kTile);
     fence_async_smem();
   }
   __syncwarp();
@@ -517,12 +518,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (; i < n; ++i) {
         const int q = (first + tile) * kTile, valid = lq - q, sa = i % kFirst, sb = i % kSecond;
         const int64_t at = (int64_t)h * a.total_q + place.q0 + q;
+        const int skip = a.causal ? max(0, -shift - q) : 0;  // queries that see no key
         // rows past the sequence: P = exp2(-inf) = 0
-        if (!load_stage<DP, true>(sq + sa * L::kTileBytes, &q_map, h, place.q0 + q, valid, &s.a_full[sa], &s.a_empty[sa],
+        if (!load_stage<DP, true>(sq + sa * L::kTileBytes, &q_map, h, place.q0 + q, skip, valid, &s.a_full[sa], &s.a_empty[sa],
                                   (i / kFirst) & 1, &s.tail, tails, a.lse2 + at, s.lse2[sa], -INFINITY, kBf16 ? 0.f : kUp))
           break;
         ++a_loads;
-        if (!load_stage<DP, true>(sg + sb * L::kTileBytes, &g_map, h, place.q0 + q, valid, &s.b_full[sb], &s.b_empty[sb],
+        if (!load_stage<DP, true>(sg + sb * L::kTileBytes, &g_map, h, place.q0 + q, skip, valid, &s.b_full[sb], &s.b_empty[sb],
                                   (i / kSecond) & 1, &s.tail, tails, a.delta + at, s.delta[sb], 0.f))
           break;
         if (++tile == per_head) {
@@ -719,11 +721,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (; j < n; ++j) {
         const int valid = lk - j * kTile, sa = j % kFirst, sb = j % kSecond;
         const int64_t k = place.k0 + (int64_t)j * kTile;
-        if (!load_stage<DP, true>(sk + sa * L::kTileBytes, &k_map, m, k, valid, &s.a_full[sa], &s.a_empty[sa],
+        if (!load_stage<DP, true>(sk + sa * L::kTileBytes, &k_map, m, k, 0, valid, &s.a_full[sa], &s.a_empty[sa],
                                   (j / kFirst) & 1, &s.tail, tails))
           break;
         ++a_loads;
-        if (!load_stage<DP, false>(sv + sb * L::kTileBytes, &v_map, m, k, valid, &s.b_full[sb], &s.b_empty[sb],
+        if (!load_stage<DP, false>(sv + sb * L::kTileBytes, &v_map, m, k, 0, valid, &s.b_full[sb], &s.b_empty[sb],
                                    (j / kSecond) & 1, &s.tail, tails))
           break;
       }

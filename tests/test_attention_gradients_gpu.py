@@ -160,3 +160,25 @@ def test_long_tail_in_fp16(cuda, dim, seqs, queries, keys):
     # keys / 16 steps
     tol = 2 * 2.0 ** -11 + 26 * 2.0 ** -23 + 2.0 ** -22 + keys / 16 * 2.0 ** -23
     assert float((out.double() / (64 * tail / (1 + tail)) - 1).abs().max()) <= tol
+
+
+@pytest.mark.parametrize('dtype', [F16, BF16])
+@pytest.mark.parametrize('dim', [64, 128])
+@pytest.mark.parametrize('lens_q,lens_k', [([300], [100]), ([129, 40, 260], [1, 40, 259]), ([200], [0]), ([3], [1])])
+def test_queries_that_see_nothing_pass_nothing(cuda, dtype, dim, lens_q, lens_k):
+    """Causal, more queries than keys: the first see no key, and whatever they and their gradients hold, NaN included,
+    nobody else's gradient shows it and theirs is 0."""
+    q, k, v, g, gl = make(dtype, 4, 2, dim, lens_q, lens_k, seed=dim + len(lens_q))
+    a = 0
+    for nq, nk in zip(lens_q, lens_k):
+        for t in (q, g):
+            t[a:a + max(0, nq - nk)] = math.nan
+        gl[:, a:a + max(0, nq - nk)] = math.nan
+        a += nq
+    for t in (q, k, v):
+        t.requires_grad_(True)
+    out, lse = packed_attention(q, k, v, offsets(lens_q), offsets(lens_k), causal=True, return_lse=True)
+    got = torch.autograd.grad((out, lse), (q, k, v), (g, gl))
+    value, tol = gradients(q.detach(), k.detach(), v.detach(), lens_q, lens_k, True, dim ** -0.5, g, gl)
+    for name, x in zip(('dq', 'dk', 'dv'), got):
+        assert bool(torch.isfinite(x).all()) and bool(((x.double() - value[name]).abs() <= tol[name]).all()), name

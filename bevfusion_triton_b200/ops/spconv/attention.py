@@ -169,6 +169,14 @@ class SparseSelfAttention(SparseModule):
         self.q_weight = nn.Parameter(torch.ones(dim)) if qk_norm else None
         self.k_weight = nn.Parameter(torch.ones(dim)) if qk_norm else None
 
+    def _apply(self, fn, recurse=True):
+        """Moves ``inv_freq`` along with the parameters, so that no call has to (a copy from the host cannot be
+        captured into a graph)."""
+        super()._apply(fn, recurse)
+        if not self.norm.weight.is_meta:  # there its values would be lost
+            self.inv_freq = self.inv_freq.to(self.norm.weight.device)
+        return self
+
     def forward(self, input: SparseConvTensor) -> SparseConvTensor:
         assert isinstance(input, SparseConvTensor)
         feats, h, m = input.features, self.heads, self.kv_heads

@@ -72,3 +72,31 @@ def test_after_a_submanifold_convolution(cuda):
     # the convolution's sums over 27 sites and the products of the layer may be blocked otherwise: fp16 roundings
     diff = (both[indices[mixed, 0] == 0].double() - alone.double()).abs().max()
     assert diff <= 2.0 ** -6 * alone.double().abs().max()
+
+
+@pytest.mark.parametrize('train', [False, True])
+def test_first_call_captured(cuda, train):
+    """The layer's first call may be the captured one (after the library handles of its products are there); replays
+    take new features and, training, draw new masks."""
+    torch.manual_seed(4)
+    indices, feats = scan(2, (60, 45), 32, 3)
+    feats = feats.half()
+    make = lambda: SparseSelfAttention(32, 2, dropout=0.5).cuda().half().train(train)  # noqa: E731
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side), torch.no_grad():  # another layer of the same shape: cuBLAS sets itself up
+        make()(SparseConvTensor(feats, indices, [8, 30, 30], 2))
+    torch.cuda.synchronize()
+    layer, graph = make(), torch.cuda.CUDAGraph()
+    with torch.no_grad(), torch.cuda.graph(graph):
+        y = layer(SparseConvTensor(feats, indices, [8, 30, 30], 2)).features
+    seen = []
+    for step in range(2):
+        feats.add_(0.25 if step else 0.0)
+        graph.replay()
+        seen.append(y.clone())
+        if not train:
+            with torch.no_grad():
+                assert torch.equal(y, layer(SparseConvTensor(feats, indices, [8, 30, 30], 2)).features)
+    if train:  # a dropped value leaves the feature itself
+        kept = [s != f for s, f in zip(seen, (feats - 0.25, feats))]
+        assert not torch.equal(kept[0], kept[1])

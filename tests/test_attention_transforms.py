@@ -1,10 +1,12 @@
 """Function transforms over the attention-block operators, on the CPU: kernels of
-a stand-in library behind the operators' own autograd kernels."""
+a stand-in library behind the operators' own autograd kernels.  And the module's
+own transform, its moves."""
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd
 
 from bevfusion_triton_b200._lib import ops
+from bevfusion_triton_b200.ops.spconv import SparseSelfAttention
 
 
 @pytest.fixture
@@ -75,3 +77,15 @@ def test_reverse_mode_through_the_stand_in(stand_in):
     x = x.clone().requires_grad_(True)
     (dx,) = torch.autograd.grad(f(x, r).sum(), x)
     assert torch.equal(dx, torch.full_like(x, 3.0))
+
+
+def test_module_moves_its_frequencies():
+    """They go where the parameters go, keep their fp32 values under .half(), and do not get lost on meta."""
+    layer = SparseSelfAttention(64, 4)
+    freq = layer.inv_freq.clone()
+    moved = []
+    layer.inv_freq = type('Spy', (), {'to': lambda self, device: moved.append(device) or freq})()
+    layer.half()
+    assert moved == [torch.device('cpu')] and layer.inv_freq is freq and 'inv_freq' not in layer.state_dict()
+    layer.to('meta')
+    assert layer.inv_freq is freq and torch.equal(layer.to_empty(device='cpu').inv_freq, freq)

@@ -12,9 +12,6 @@
 
 namespace bfb {
 
-BFB_DEBUG_COUNTER();
-BFB_DEBUG_READER(debug_violations_attention)
-
 namespace {
 
 using Attn = attn::Args;

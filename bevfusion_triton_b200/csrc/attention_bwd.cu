@@ -41,6 +41,10 @@
 #include "attention.cuh"
 
 namespace bfb {
+
+BFB_DEBUG_COUNTER();
+BFB_DEBUG_READER(debug_violations_attention_bwd)
+
 namespace attn {
 
 namespace {
@@ -268,7 +272,7 @@ __device__ __forceinline__ float lift(float bound) {
 // and signals `full` (two arrivals).  The values are fetched before the wait, all at once: one after
 // another behind it, their latencies were most of a step.
 template <int DP, bool kClear>
-__device__ __forceinline__ bool load_stage(uint8_t* dst, const CUtensorMap* map, int head, int64_t row, int skip, int valid,
+__device__ __forceinline__ bool load_stage(uint8_t* dst, const CUtensorMap* map, int head, int64_t row, int64_t rows, int skip, int valid,
                                            uint64_t* full, uint64_t* empty, uint32_t parity, uint64_t* tail,
                                            uint32_t& tails, const float* src = nullptr, float* values = nullptr,
                                            float past = 0.f, float add = 0.f) {
@@ -277,7 +281,7 @@ __device__ __forceinline__ bool load_stage(uint8_t* dst, const CUtensorMap* map,
   float x[4];
   if (src) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) x[e] = lane + 32 * e < valid ? add - src[lane + 32 * e] : past;
+    for (int e = 0; e < 4; ++e) x[e] = lane + 32 * e < valid && !BFB_BAD(row + lane + 32 * e < rows) ? add - src[lane + 32 * e] : past;
   }
   if (lane == 0) ok = bar_wait(empty, parity ^ 1, &g_timeouts);
   if (!__shfl_sync(0xffffffffu, ok, 0)) return false;
@@ -451,7 +455,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (ok && (n == 0 || bar_wait_warp(&s.done, 0, &g_timeouts))) {
       tc_fence_after();
       T* out = static_cast<T*>(wg ? a.dk : a.dv) + ((place.k0 + j) * a.kv_heads + m) * a.dim;
-      write_row<T>((wg ? tdk : tdv) + lanes, out, 0, DP, a.dim, j < place.room, n == 0 || j >= lk,
+      write_row<T>((wg ? tdk : tdv) + lanes, out, 0, DP, a.dim, j < place.room && !BFB_BAD(place.k0 + j < a.total_k), n == 0 || j >= lk,
                    kBf16 ? 1.f : wg ? 1.f / f : kDown);
     }
   } else {
@@ -520,11 +524,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int64_t at = (int64_t)h * a.total_q + place.q0 + q;
         const int skip = a.causal ? max(0, -shift - q) : 0;  // queries that see no key
         // rows past the sequence: P = exp2(-inf) = 0
-        if (!load_stage<DP, true>(sq + sa * L::kTileBytes, &q_map, h, place.q0 + q, skip, valid, &s.a_full[sa], &s.a_empty[sa],
+        if (!load_stage<DP, true>(sq + sa * L::kTileBytes, &q_map, h, place.q0 + q, a.total_q, skip, valid, &s.a_full[sa], &s.a_empty[sa],
                                   (i / kFirst) & 1, &s.tail, tails, a.lse2 + at, s.lse2[sa], -INFINITY, kBf16 ? 0.f : kUp))
           break;
         ++a_loads;
-        if (!load_stage<DP, true>(sg + sb * L::kTileBytes, &g_map, h, place.q0 + q, skip, valid, &s.b_full[sb], &s.b_empty[sb],
+        if (!load_stage<DP, true>(sg + sb * L::kTileBytes, &g_map, h, place.q0 + q, a.total_q, skip, valid, &s.b_full[sb], &s.b_empty[sb],
                                   (i / kSecond) & 1, &s.tail, tails, a.delta + at, s.delta[sb], 0.f))
           break;
         if (++tile == per_head) {
@@ -567,15 +571,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, mine = lanes + wg * kHalf;
     const float2 c2 = make_float2(a.scale * kLog2e, a.scale * kLog2e);
     const int64_t at = (int64_t)h * a.total_q + place.q0 + i;
-    const float lse2 = i < lq ? a.lse2[at] : INFINITY;
-    const float delta = i < lq ? a.delta[at] : 0.f;
+    const bool in_part = i < lq && !BFB_BAD(place.q0 + i < a.total_q);
+    const float lse2 = in_part ? a.lse2[at] : INFINITY;
+    const float delta = in_part ? a.delta[at] : 0.f;
     float f = 1.f;
     if (!kBf16 && n > 0) {
       float v = 0.f;
 #pragma unroll 4
       for (int j = threadIdx.x; j < min(lk, n * kTile); j += 256) v = fmaxf(v, a.norm_v[(int64_t)m * a.total_k + place.k0 + j]);
       v = largest(s, v, 0.f).x;
-      if (i < lq) f = lift(fabsf(a.scale) * a.norm_g[at] * v + fabsf(delta));
+      if (in_part) f = lift(fabsf(a.scale) * a.norm_g[at] * v + fabsf(delta));
     }
     const float down = kBf16 ? 1.f : f * kDown, off = (kBf16 ? 0.f : kUp) - lse2;
     const float2 off2 = make_float2(off, off), scale2 = make_float2(a.scale * down, a.scale * down),
@@ -644,14 +649,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     s.delta[wg][row] = lacks.x + lacks.y;
     warpgroups_sync();
     // of a row that sees no key nothing is read
-    const bool live = i < lq && lse2 != INFINITY;
+    const bool live = in_part && lse2 != INFINITY;
     const float e = live ? s.delta[0][row] + s.delta[1][row] - (a.dlse ? f * a.scale * a.dlse[at] : 0.f) : 0.f;
     if (ok && live && wg == 0) a.delta[at] = delta + e / f;
     if (ok && (n == 0 || bar_wait_warp(&s.done, 0, &g_timeouts))) {
       tc_fence_after();
       T* out = static_cast<T*>(a.dq) + ((place.q0 + i) * a.heads + h) * a.dim;
       const int col0 = wg * (DP / 2);
-      write_row<T>(tdq + lanes + col0, out, col0, DP / 2, a.dim, i < lq, n == 0, 1.f / f, tpk + lanes + col0,
+      write_row<T>(tdq + lanes + col0, out, col0, DP / 2, a.dim, in_part, n == 0, 1.f / f, tpk + lanes + col0,
                    kBf16 ? e : e * kDown);
     }
   } else {
@@ -721,11 +726,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (; j < n; ++j) {
         const int valid = lk - j * kTile, sa = j % kFirst, sb = j % kSecond;
         const int64_t k = place.k0 + (int64_t)j * kTile;
-        if (!load_stage<DP, true>(sk + sa * L::kTileBytes, &k_map, m, k, 0, valid, &s.a_full[sa], &s.a_empty[sa],
+        if (!load_stage<DP, true>(sk + sa * L::kTileBytes, &k_map, m, k, a.total_k, 0, valid, &s.a_full[sa], &s.a_empty[sa],
                                   (j / kFirst) & 1, &s.tail, tails))
           break;
         ++a_loads;
-        if (!load_stage<DP, false>(sv + sb * L::kTileBytes, &v_map, m, k, 0, valid, &s.b_full[sb], &s.b_empty[sb],
+        if (!load_stage<DP, false>(sv + sb * L::kTileBytes, &v_map, m, k, a.total_k, 0, valid, &s.b_full[sb], &s.b_empty[sb],
                                    (j / kSecond) & 1, &s.tail, tails))
           break;
       }

@@ -31,6 +31,10 @@
 #include "attention.cuh"
 
 namespace bfb {
+
+BFB_DEBUG_COUNTER();
+BFB_DEBUG_READER(debug_violations_attention_fwd)
+
 namespace attn {
 
 namespace {
@@ -290,9 +294,10 @@ __global__ void __launch_bounds__(256, 2)
       tc_fence_after();
     }
     if (ok) {
+      const bool live = i < lq && !BFB_BAD(place.q0 + i < a.total_q);
       T* out = static_cast<T*>(a.out) + ((place.q0 + i) * a.heads + h) * a.dim;
-      write_o<T, DP>(to + lanes, sum, out, a.dim, n > 0, i < lq);
-      if (i < lq) a.lse[(int64_t)h * a.total_q + place.q0 + i] = lse_of(top, sum);
+      write_o<T, DP>(to + lanes, sum, out, a.dim, n > 0, live);
+      if (live) a.lse[(int64_t)h * a.total_q + place.q0 + i] = lse_of(top, sum);
     }
   } else {
     regs_shrink<56>();
@@ -466,7 +471,7 @@ __global__ void __launch_bounds__(512, 1)
     }
     s.sum[t][row] = sum;
     bar_arrive_warp(&s.sums[t]);
-    if (i < lq) a.lse[(int64_t)h * a.total_q + place.q0 + i] = lse_of(top, sum);
+    if (i < lq && !BFB_BAD(place.q0 + i < a.total_q)) a.lse[(int64_t)h * a.total_q + place.q0 + i] = lse_of(top, sum);
   } else if (warp < 12) {
     regs_shrink<80>();
     const int row = threadIdx.x & (kTile - 1);
@@ -493,7 +498,7 @@ __global__ void __launch_bounds__(512, 1)
         break;
       tc_fence_after();
       T* out = static_cast<T*>(a.out) + ((place.q0 + i) * a.heads + h) * a.dim;
-      write_o<T, DP>(to + lanes + t * DP, s.sum[t][row], out, a.dim, steps > 0, i < lq);
+      write_o<T, DP>(to + lanes + t * DP, s.sum[t][row], out, a.dim, steps > 0, i < lq && !BFB_BAD(place.q0 + i < a.total_q));
     }
   } else {
     regs_shrink<64>();

@@ -27,6 +27,10 @@
 #include "attention.cuh"
 
 namespace bfb {
+
+BFB_DEBUG_COUNTER();
+BFB_DEBUG_READER(debug_violations_attention_rows)
+
 namespace attn {
 
 namespace {
@@ -332,6 +336,8 @@ __global__ void __launch_bounds__(kThreads, 2)
         total_sum += w[i] * sum_s[hh + i * kHeads][r];
       }
       const bool whole = tiles == x.tiles;
+      // a group that a cut goes through is the first of its block or its last, so that a block has two records at most
+      if (BFB_BAD(whole || pos == begin || pos + tiles == end)) continue;
       float* rec = records + (((int64_t)2 * blockIdx.x + (pos == begin ? 0 : 1)) * kHeads + hh) * record_floats<DP>();
       const int h = (m0 + hh) * group + (int)(rr % group);
       const int64_t row = x.q0 + rr / group;
@@ -350,7 +356,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         }
         if (!whole) {
           *reinterpret_cast<float4*>(rec + r * DP + col) = v;
-        } else if (rr < rows && col < a.dim) {
+        } else if (rr < rows && col < a.dim && !BFB_BAD(row < a.total_q && h < a.heads)) {
           uint2 packed = make_uint2(0u, 0u);
           if (inv != 0.f) packed = make_uint2(pack2<T>(v.x * inv, v.y * inv), pack2<T>(v.z * inv, v.w * inv));
           *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (row * a.heads + h) * a.dim + col) = packed;
@@ -409,6 +415,7 @@ __global__ void __launch_bounds__(128) join_kernel(const __grid_constant__ Args 
     const int64_t c0 = first / per, c1 = (first + x.tiles - 1) / per;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (c0 == c1) return;  // written by its block
+    if (BFB_BAD(c0 >= 0 && c1 < blocks)) return;
     for (int64_t c = c0; c <= c1; c += 32) {
       const int n = (int)min((int64_t)32, c1 + 1 - c);
       // at the end of a block's stretch where it began before the group, else at its start

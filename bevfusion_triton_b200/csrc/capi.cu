@@ -75,7 +75,9 @@ extern "C" int bfb_debug_violations(uint64_t* count, int reset) {
   BFB_TRY(bfb::debug_violations_spconv(count, reset));
   BFB_TRY(bfb::debug_violations_spconv_conv(count, reset));
   BFB_TRY(bfb::debug_violations_token_ops(count, reset));
-  BFB_TRY(bfb::debug_violations_attention(count, reset));
+  BFB_TRY(bfb::debug_violations_attention_fwd(count, reset));
+  BFB_TRY(bfb::debug_violations_attention_bwd(count, reset));
+  BFB_TRY(bfb::debug_violations_attention_rows(count, reset));
   BFB_TRY(bfb::debug_violations_capi(count, reset));
   return BFB_OK;
 }

@@ -68,7 +68,9 @@ int debug_violations_scatter(uint64_t* v, int reset);
 int debug_violations_spconv(uint64_t* v, int reset);
 int debug_violations_spconv_conv(uint64_t* v, int reset);
 int debug_violations_token_ops(uint64_t* v, int reset);
-int debug_violations_attention(uint64_t* v, int reset);
+int debug_violations_attention_fwd(uint64_t* v, int reset);
+int debug_violations_attention_bwd(uint64_t* v, int reset);
+int debug_violations_attention_rows(uint64_t* v, int reset);
 int debug_violations_capi(uint64_t* v, int reset);
 
 // A status armed by bfb_debug_inject_status for the next calls of the main

@@ -337,6 +337,7 @@ __global__ void __launch_bounds__(kThreads, kForwardBlocks) rotary_forward_kerne
       x0[i].zero();
       x1[i].zero();
       if (i >= a.steps || i * a.k + me.token >= count) continue;
+      if (BFB_BAD(t0 + i * a.k + me.token < a.tokens && (me.c0 < 0 || me.head < heads))) continue;
       const T* from = x + (t0 + i * a.k) * row;
       if (me.c0 >= 0) x0[i].load(from + me.c0);
       if (me.c1 >= 0) x1[i].load(from + me.c1);
@@ -415,6 +416,7 @@ __global__ void __launch_bounds__(kThreads, kBackBlocks) rotary_backward_kernel(
       g0[i].zero();
       g1[i].zero();
       if (i >= a.steps || i * a.k + me.token >= count) continue;
+      if (BFB_BAD(t0 + i * a.k + me.token < a.tokens && (me.c0 < 0 || me.head < heads))) continue;
       const T* gr = g + (t0 + i * a.k) * out_row;
       if (me.c0 >= 0) g0[i].load(gr + me.c0);
       if (me.c1 >= 0) g1[i].load(gr + me.c1);
@@ -491,6 +493,7 @@ __global__ void __launch_bounds__(kThreads, kBackBlocks) rotary_backward_kernel(
   }
   __syncthreads();
   const int all = a.heads[0] + a.heads[1];
+  if (BFB_BAD(gridDim.x * gridDim.y <= (unsigned)kMostPartials)) return;
   for (int i = threadIdx.x; i < 2 * a.dim; i += blockDim.x) {
     const int side = i >= a.dim, c = i - side * a.dim;
     float v = 0.f;

@@ -16,6 +16,6 @@ Beside them, without a reference counterpart: attention over active sites
 All kernels live in ``libbfb_b200.so`` (C ABI, include/bfb_b200.h); torch
 custom ops in ``_bfb_torch.so`` wrap it.  There is no CPU or Triton path.
 """
-from ._lib import load_native, native_paths  # noqa: F401
+from ._lib import gave_up_waits, load_native, native_paths  # noqa: F401
 
-__all__ = ['load_native', 'native_paths']
+__all__ = ['load_native', 'native_paths', 'gave_up_waits']

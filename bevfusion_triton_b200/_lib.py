@@ -58,3 +58,22 @@ def bev_pool_plan_bytes(n: int, B: int, D: int, H: int, W: int) -> int:
     if st != 0:
         raise ValueError(f'bev_pool geometry (n={n}, B={B}, D={D}, H={H}, W={W}) is refused (status {st})')
     return plan.value
+
+
+def gave_up_waits(device=None, reset: bool = False) -> int:
+    """How many bounded waits inside the tensor-core kernels (sparse convolution
+    and packed attention) have given up on ``device`` (default: the current
+    one), since the library was loaded or since ``reset``.  0 in a correct run;
+    otherwise results of the calls in between are not to be used, although the
+    calls themselves returned.  Waits for the device's work."""
+    lib = load_native()
+    total = 0
+    with torch.cuda.device(device):
+        torch.cuda.synchronize()
+        for name in ('bfb_spconv_timeouts', 'bfb_attention_timeouts'):
+            count = ctypes.c_uint64(0)
+            status = getattr(lib, name)(ctypes.byref(count), int(reset))
+            if status != 0:
+                raise RuntimeError(f'{name} failed (status {status})')
+            total += count.value
+    return total

@@ -38,14 +38,14 @@ int check_args(const Attn& a, int dtype) {
 // keys: up to two of its 16-row tiles for the average sequence and key head.
 // Split kernel / tile kernel, us, 32/8 heads of 128, bf16, causal, by rows (queries x query heads of a key head):
 //   sequences x keys     4 rows         32            64            128
-//       4 x   128      13.3 /  12    13.7 /  12    14.2 /  12    18.5 /  12
-//       4 x 20000        73 / 261     116 / 260     202 / 261     369 / 261
-//      32 x   128        15 /  50      26 /  53      40 /  54      63 /  55
-//      32 x  8000       175 / 747     332 / 748     644 / 748    1297 / 762
-// Heads of 64 cross between 32 and 64 (32 x 128: 20 / 23 at 32, 32 / 23 at 64; 32 x 8000: 327 / 352 at 64), so the limit
-// stays below what 128 alone would take.  Lengths are on the device, so the rule sees their average: a batch of one long
-// prompt and many single queries can get the split kernel for all of it.  Such mixes were not timed; where every sequence
-// has 256 rows the split kernel takes 2546 us for 747 (32 x 8000).  Two calls avoid it.
+//       4 x   128        12 /  12      12 /  12      12 /  12      16 /  12
+//       4 x 20000        72 / 261     116 / 261     202 / 261     368 / 260
+//      32 x   128        13 /  50      23 /  53      38 /  54      60 /  55
+//      32 x  8000       172 / 746     332 / 748     644 / 747    1310 / 747
+// Heads of 64 cross between 32 and 64 (32 x 128: 20 / 23 at 32, 34 / 23 at 64; 32 x 8000: 326 / 367 at 64), so the limit
+// stays below what 128 alone would take.  Lengths are on the device, so the rule sees their average, and one kernel takes
+// a whole batch: a prompt of 4000 with 100 single queries on 2000 keys each 825 us (tiles; apart 136 + 142), with 600 on
+// 500 keys 2195 us (split; apart 136 + 285).  Two calls avoid it.
 bool few_rows(int64_t total_q, int64_t heads, int64_t kv_heads, int64_t seqs) {
   return total_q * (heads / kv_heads) <= 32 * seqs;
 }

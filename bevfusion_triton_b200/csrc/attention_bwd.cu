@@ -2,14 +2,14 @@
 //   P = exp2(c S - lse2),  dS = P (scale dP - scale delta)
 // one kernel owns key tiles and sums dK and dV over the query tiles and the
 // query heads of its key head, another owns query tiles and sums dQ over the
-// key tiles.  That computes S and dP twice (seven products for the five that
-// one kernel with dQ in atomics would need), but every sum has a fixed order,
+// key tiles.  That computes S and dP twice (eight products, with the P K below, for
+// the five that one kernel with dQ in atomics would need), but every sum has a fixed order,
 // no fp32 copy of dQ goes through memory, and nothing has to be cleared first.
 //
 // Both keep their sums in tensor memory over the whole walk.  dS (and P for
 // dV) are rounded to 16 bits and stay in tensor memory, over the scores they
 // came from, as the next product's first operand (the rounding of dS is most
-// of what dQ and dK lose: relative errors of 0.0025 in bf16 and 0.0003 in fp16
+// of what dQ and dK lose: relative errors of 0.0024 in bf16 and 0.0003 in fp16
 // against 64 bits, where fp32 inside has 0.0017 and 0.0002); each 128 x 128 step is
 // worked by two warpgroups, one per 64 columns, with 64 values per thread.
 //
@@ -31,9 +31,9 @@
 // dQ at the end; delta + e is left for the dK and dV kernel, which runs second.
 // That costs the dQ kernel a fourth product.
 //
-// Measured, one sequence of 8192 tokens, full.  8/2 heads of 128, bf16: dQ 374 us
-// (tensor pipe 55 % busy, special functions 43 %), dK and dV 460 us (61 and 36
-// %); 8 heads of 64, fp16: 315 us (32 and 50 %) and 424 us (32 and 37 %).  The
+// Measured, one sequence of 8192 tokens, full.  8/2 heads of 128, bf16: dQ 456 us
+// (tensor pipe 61 % busy, special functions 36 %), dK and dV 440 us (63 and 37
+// %); 8 heads of 64, fp16: 407 us (33 and 39 %) and 423 us (32 and 37 %).  The
 // chain of a step bounds them, with one block to an SM.
 #include <algorithm>
 #include <cfloat>
@@ -67,7 +67,8 @@ struct Layout {
   static constexpr int kTileBytes = kTile * DP * 2;
   static constexpr int kPanel = kTile * 128;
   // dV's product starts on the first half of P while the second is formed: with heads of 128, where a product takes
-  // as long as that (causal, 0.7 - 4 k tokens, 16/4 heads: 295 -> 285 us; with 64 the arrivals cost more, 83 -> 85)
+  // as long as that (causal, 0.7 - 4 k tokens, 16/4 heads: 295 -> 285 us; with 64 the arrivals cost more, 83 -> 85);
+  // dQ's P K in the same way (forward and backward 825 -> 814)
   static constexpr bool kSplit = DP == 128;
   static constexpr int kTiles = 7;  // two resident tiles, three of the first ring, two of the second
 };

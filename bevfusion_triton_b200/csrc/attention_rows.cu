@@ -20,7 +20,7 @@
 // the tensor pipe is not what bounds this.
 //
 // 24 streams of one query, caches of up to 30 k keys, 32/8 heads of 128, bf16 (479 MB): 114 us, 4.2 TB/s; a plain
-// sum over as many bytes reaches 5.5.  Three stages and two blocks to an SM: two stages 112, three blocks 123
+// sum over as many bytes reaches 5.0.  Three stages and two blocks to an SM: two stages 112, three blocks 123
 // (registers spill), eight warps and key heads in one block 118, one key head at a time 118.
 #include <algorithm>
 

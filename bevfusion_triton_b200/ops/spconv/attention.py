@@ -59,12 +59,16 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     Returns out [queries, heads, dim] (and, with ``return_lse``, the fp32
     log of each query's sum of exponentials, [heads, queries]).  A query that
     sees no key and a row that no sequence holds get 0 (and -inf), and pass
-    no gradient.  Rows of ``k`` and ``v`` outside every sequence and past
-    ``kv_lengths`` may hold anything; a non-finite ``v`` inside a sequence may
-    reach all queries of that sequence.  Gradients are deterministic; the
-    probabilities and their gradients are rounded to the inputs' type inside,
-    which leaves dq and dk relative errors near 0.0025 in bf16 and 0.0003 in
-    fp16 (0.0017 and 0.0002 with fp32 inside).
+    no gradient, whatever they and their gradients hold.  Rows of ``k`` and
+    ``v`` outside every sequence and past ``kv_lengths`` may hold anything; a
+    non-finite ``v`` inside a sequence may reach all queries of that sequence,
+    and a non-finite value of a query that sees keys, of a key or of a gradient
+    all gradients of the sequence, hidden or not.  Gradients are deterministic;
+    the probabilities and their gradients are rounded to the inputs' type
+    inside (in fp16 times powers of two that keep them out of the subnormal
+    numbers), which leaves dq and dk relative errors near 0.0024 in bf16 and
+    0.0003 in fp16 (0.0017 and 0.0002 with fp32 inside).  Second derivatives
+    and forward mode are refused.
     """
     _require_cuda(q, k, v, cu_seqlens_q)
     if scale is None:

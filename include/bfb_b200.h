@@ -494,11 +494,16 @@ int bfb_spconv_timeouts(uint64_t* count, int reset);
  * exp(scale q k^T).  A query that sees no key, and a row of no sequence, gets
  * out = 0 and lse = -inf.  Keys of no sequence and rows of k and v past
  * kv_lengths may hold anything, NaN included; a non-finite v of a sequence may
- * reach every query of that sequence, also those that do not see it.
+ * reach every query of that sequence, also those that do not see it.  The
+ * workspace's size depends on the sizes alone (backward: three floats for each
+ * query and head and one for each key and key head).
  *
  * Backward: gradients of q, k and v (contiguous; zero where a row takes no
  * part) from those of out and (nullable) lse.  Deterministic: the sums over
- * queries, keys and the query heads of a key head have a fixed order.
+ * queries, keys and the query heads of a key head have a fixed order.  Queries
+ * that see no key may hold anything, and so may their gradients; a non-finite
+ * value of another query, of a key or of a gradient may reach every gradient of
+ * its sequence.
  * ---------------------------------------------------------------------- */
 int bfb_packed_attention_workspace_size(int64_t total_q, int64_t total_k, int64_t heads, int64_t kv_heads,
                                         int64_t dim, int64_t seqs, int backward, size_t* bytes);

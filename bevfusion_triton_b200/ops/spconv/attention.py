@@ -66,8 +66,8 @@ def packed_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     all gradients of the sequence, hidden or not.  Gradients are deterministic;
     the probabilities and their gradients are rounded to the inputs' type
     inside (in fp16 times powers of two that keep them out of the subnormal
-    numbers), which leaves dq and dk relative errors near 0.0024 in bf16 and
-    0.0003 in fp16 (0.0017 and 0.0002 with fp32 inside).  Second derivatives
+    numbers), which leaves dq and dk relative errors of up to 0.0026 in bf16
+    and 0.0003 in fp16 (0.0017 and 0.0002 with fp32 inside).  Second derivatives
     and forward mode are refused.
     """
     _require_cuda(q, k, v, cu_seqlens_q)

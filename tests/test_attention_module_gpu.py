@@ -100,3 +100,25 @@ def test_first_call_captured(cuda, train):
     if train:  # a dropped value leaves the feature itself
         kept = [s != f for s, f in zip(seen, (feats - 0.25, feats))]
         assert not torch.equal(kept[0], kept[1])
+
+
+@pytest.mark.parametrize('rows', [0, 1, 2])
+@pytest.mark.parametrize('batch', [1, 3])
+def test_hardly_any_sites(cuda, rows, batch):
+    """No site, one, and one in each of two samples in descending order: a site that sees itself alone gets its value's
+    projection; a training step gives finite gradients."""
+    torch.manual_seed(5)
+    layer = SparseSelfAttention(32, 2, dropout=0.1).cuda().half()
+    indices = torch.tensor([[min(batch - 1, 1 - r), r, 4, 5] for r in range(rows)], dtype=torch.int32,
+                           device='cuda').view(rows, 4)
+    feats = torch.randn(rows, 32, device='cuda').half().requires_grad_(True)
+    y = layer(SparseConvTensor(feats, indices, [8, 30, 30], batch)).features
+    y.float().sum().backward()
+    grads = [feats.grad] + [p.grad for p in layer.parameters()]
+    assert y.shape == feats.shape and all(bool(torch.isfinite(t).all()) for t in [y, *grads])
+    if batch > 1:
+        with torch.no_grad():
+            got = layer.eval()(SparseConvTensor(feats, indices, [8, 30, 30], batch)).features
+            value = layer.qkv(layer.norm(feats))[:, 64:]
+            want = feats + layer.proj(value)
+        assert torch.equal(got, want)
